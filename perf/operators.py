@@ -1,0 +1,494 @@
+"""The workloads that measure the paged 4-bit key/value cache, with each operator's plain form.
+
+Three operators make up the cached half of a decoder layer, after the fused residual add +
+RMSNorm + Q/K/V projection with the rotary embedding:
+
+* ``plan``    block tables and slot maps of a batch, from the requests' lengths and a free list;
+* ``store``   keys and values quantised to 4 bits into their slots, and read back as numbers;
+* ``attend``  causal attention of the new tokens over the 4-bit cache.
+
+``own`` chooses who computes: elementary torch operations in 32 bits, or the package's calls.
+
+The cache's bytes.  A block of P tokens of one KV head is P / 16 records of 16 tokens; a record
+holds the keys' codes, the values' codes, then one (scale, minimum) pair of 16-bit numbers per
+token and group of dims, for the keys and for the values: 16 D + 128 D / group bytes.  A code c
+stands for scale * c + minimum.
+  keys    token t, dim d = 32 i + 8 c + 2 j + b sits in byte t D/2 + c D/8 + 4 i + 2 b + j / 2
+          (low half of the byte for even j)
+  values  token t = 8 h + 2 c + b, dim d = 32 i + 4 g + j sits in the 16-bit word
+          (h, g, c, i, b) for D = 128 and (g, c, h, i, b) for D = 64, bits 4 j .. 4 j + 3
+"""
+import functools
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+# ------------------------------------------------------------------ cases
+# Shapes are the framework's own decode and prompt configurations (query heads over KV heads:
+# 32 / 8, 28 / 4, 64 / 8, heads of 128) and small generic ones.
+def listed():
+    return [
+        # A serving step's bookkeeping: every request adds one token, few need a new block.
+        dict(name="plan decode 64", op="plan", requests=64, lo=1, hi=4000, new=1, block=16, short=0, lens=1),
+        # A scheduler step that admits many prompts beside running requests, with too few free
+        # blocks for the last of them.
+        dict(name="plan mixed 700", op="plan", requests=700, lo=0, hi=4096, new=129, block=32, short=40, lens=2),
+        # One decode step of four requests (8 KV heads of 128): latency only.
+        dict(name="store decode 4", op="store", batch=4, tokens=1, n_kv=8, dim=128, group=128, block=16, dtype="bf16"),
+        # A prompt's keys and values, head-major as the rotary split leaves them.
+        dict(name="store prompt 16384", op="store", batch=2, tokens=8192, n_kv=8, dim=128, group=128, block=64,
+             dtype="bf16"),
+        # An odd prompt in fp16 with small heads and fine groups.
+        dict(name="store odd 1537", op="store", batch=1, tokens=1537, n_kv=4, dim=64, group=32, block=16, dtype="fp16"),
+        # The first decode steps of one chat: a short cache, latency only.
+        dict(name="attend one 700", op="attend", requests=1, lo=700, hi=700, new_lo=1, new_hi=1, n_q=32, n_kv=8, dim=128,
+             group=128, block=16, window=0, dtype="bf16", lens=1),
+        # A full decode batch with ragged lengths.
+        dict(name="attend decode 64", op="attend", requests=64, lo=1, hi=8000, new_lo=1, new_hi=1, n_q=32, n_kv=8,
+             dim=128, group=128, block=16, window=0, dtype="bf16", lens=2),
+        # Two long documents (28 query heads on 4 KV heads, groups of 32 dims).
+        dict(name="attend long 131071", op="attend", requests=2, lo=130000, hi=131071, new_lo=1, new_hi=1, n_q=28,
+             n_kv=4, dim=128, group=32, block=64, window=0, dtype="bf16", lens=3),
+        # Multi-head attention with heads of 64 in fp16 and a sliding window.
+        dict(name="attend window 32", op="attend", requests=32, lo=50, hi=4000, new_lo=1, new_hi=1, n_q=16, n_kv=16,
+             dim=64, group=64, block=32, window=1024, dtype="fp16", lens=4),
+        # Draft tokens checked against the cache, five for each request (64 query heads on 8).
+        dict(name="attend verify 16x5", op="attend", requests=16, lo=500, hi=6000, new_lo=5, new_hi=5, n_q=64, n_kv=8,
+             dim=128, group=128, block=16, window=0, dtype="bf16", lens=5),
+        # A prompt of 4096 tokens from an empty cache.
+        dict(name="attend prompt 4096", op="attend", requests=1, lo=4096, hi=4096, new_lo=4096, new_hi=4096, n_q=32,
+             n_kv=8, dim=128, group=128, block=64, window=0, dtype="bf16", lens=6),
+        # Chunks of prompts of odd lengths over caches of odd lengths, one batch.
+        dict(name="attend chunks 4", op="attend", requests=4, lo=600, hi=12000, new_lo=1, new_hi=600, n_q=28, n_kv=4,
+             dim=128, group=64, block=16, window=0, dtype="bf16", lens=7),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, max(lo, round(math.exp(rng.uniform(math.log(lo), math.log(hi))))))
+
+
+def draw(rng):
+    while True:
+        case = _draw(rng)
+        cost = work(case)
+        if cost["bytes"] <= 2.8e8 and cost["flops"] <= 1.3e11:  # the largest listed cases
+            return case
+
+
+def _draw(rng):
+    op = rng.choice(["plan", "store", "attend", "attend", "attend"])
+    block = rng.choice([16, 32, 48, 64, 128])
+    dtype = rng.choice(["bf16", "bf16", "fp16"])
+    dim = rng.choice([64, 128, 128])
+    group = rng.choice([g for g in (32, 64, 128) if g <= dim])
+    if op == "plan":
+        return dict(op=op, requests=_log_int(rng, 1, 1500), lo=0, hi=_log_int(rng, 16, 4096),
+                    new=rng.choice([1, 1, 7, 129]), block=block, short=rng.choice([0, 0, 5]), lens=rng.randrange(1 << 20))
+    if op == "store":
+        batch = _log_int(rng, 1, 8)
+        return dict(op=op, batch=batch, tokens=_log_int(rng, 1, 16384 // batch), n_kv=rng.choice([1, 2, 4, 8]), dim=dim,
+                    group=group, block=block, dtype=dtype)
+    n_kv, ratio = rng.choice([(8, 4), (4, 7), (8, 8), (2, 16), (16, 1), (8, 2), (1, 32)])
+    kind = rng.choice(["decode", "decode", "verify", "chunk"])
+    if kind == "decode":
+        requests, new = _log_int(rng, 1, 64), 1
+        hi = _log_int(rng, 16, min(130000, 250000 // requests))
+    elif kind == "verify":
+        requests, new = _log_int(rng, 1, 16), rng.randint(2, 16)
+        hi = _log_int(rng, 64, 60000 // requests)
+    else:
+        requests = rng.randint(1, 4)
+        new = _log_int(rng, 17, 1200 // requests)
+        hi = new + _log_int(rng, 16, 24000 // requests)
+    fixed = rng.random() < 0.5
+    return dict(op="attend", requests=requests, lo=max(1, hi // 3), hi=hi, new_lo=new if fixed else 1, new_hi=new,
+                n_q=n_kv * ratio, n_kv=n_kv, dim=dim, group=group, block=block,
+                window=rng.choice([0, 0, 0, rng.randint(1, hi)]), dtype=dtype, lens=rng.randrange(1 << 20))
+
+
+def _lens(case):
+    """(tokens cached before the call, tokens added by it) of each request."""
+    rng = random.Random(case["lens"])
+    if case["op"] == "plan":
+        ctx = [rng.randint(case["lo"], case["hi"]) for _ in range(case["requests"])]
+        new = [rng.randint(1, case["new"]) for _ in ctx]
+        return ctx, new
+    total = [rng.randint(case["lo"], case["hi"]) for _ in range(case["requests"])]
+    total[rng.randrange(len(total))] = case["hi"]
+    new = [min(t, rng.randint(case["new_lo"], case["new_hi"])) for t in total]
+    return [t - n for t, n in zip(total, new)], new
+
+
+def _blocks(n, block):
+    return -(-n // block)
+
+
+def work(case):
+    if case["op"] == "plan":
+        ctx, new = _lens(case)
+        fresh = sum(_blocks(c + n, case["block"]) - _blocks(c, case["block"]) for c, n in zip(ctx, new))
+        # lengths in, starts and lengths out; free list entries in, table entries out; two ints a token
+        return {"bytes": 4 * (4 * len(ctx) + 2 * fresh + 2 * sum(new)), "flops": 0}
+    per_row = case["dim"] // 2 + 4 * (case["dim"] // case["group"])
+    if case["op"] == "store":
+        rows = 2 * case["batch"] * case["tokens"] * case["n_kv"]
+        # 16-bit numbers in, codes and parameters written and read back, 16-bit numbers out
+        return {"bytes": rows * (4 * case["dim"] + 2 * per_row) + 8 * case["batch"] * case["tokens"],
+                "flops": 10 * rows * case["dim"]}
+    ctx, new = _lens(case)
+    pairs = keys = 0
+    for c, n in zip(ctx, new):
+        seen = [min(c + j + 1, case["window"] or c + j + 1) for j in range(n)]
+        pairs += sum(seen)
+        keys += min(c + n, c + n - (c + 1 - seen[0])) if n else 0
+    return {"bytes": 2 * keys * case["n_kv"] * per_row + 4 * sum(new) * case["n_q"] * case["dim"],
+            "flops": 4 * pairs * case["n_q"] * case["dim"]}
+
+
+# ------------------------------------------------------------------ inputs
+def _int32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _heads(gen, shape, dtype):
+    """Activations with a spread and an offset that differ from channel to channel."""
+    spread = torch.exp(0.4 * torch.randn(shape[-1], generator=gen, device="cuda"))
+    offset = 0.5 * torch.randn(shape[-1], generator=gen, device="cuda")
+    return (torch.randn(shape, generator=gen, device="cuda") * spread + offset).to(dtype)
+
+
+def _quantise(x, group):
+    """(codes, scale, minimum) of rows x (..., D): codes 0..15, scale and minimum in x's type."""
+    g = x.float().unflatten(-1, (-1, group))
+    low, high = g.amin(-1), g.amax(-1)
+    scale, low = ((high - low) / 15).to(x.dtype), low.to(x.dtype)
+    s = scale.float().unsqueeze(-1)
+    code = torch.where(s > 0, ((g - low.float().unsqueeze(-1)) / s).round().clamp(0, 15), 0.0)
+    return code.to(torch.uint8).flatten(-2), scale, low
+
+
+def _key_bytes(codes):
+    """(..., 16, D) codes -> (..., 8 D) bytes."""
+    D = codes.shape[-1]
+    x = codes.reshape(*codes.shape[:-1], D // 32, 4, 2, 2, 2)  # t | i, c, j / 2, j % 2, b
+    n = x.dim()
+    x = x.permute(*range(n - 5), n - 4, n - 5, n - 1, n - 3, n - 2)  # t | c, i, b, j / 2, j % 2
+    return (x[..., 0] | (x[..., 1] << 4)).flatten(-5)
+
+
+def _value_bytes(codes):
+    """(..., 16, D) codes -> (..., 8 D) bytes."""
+    D = codes.shape[-1]
+    x = codes.reshape(*codes.shape[:-2], 2, 4, 2, D // 32, 8, 2, 2)  # h, c, b, i, g, j / 2, j % 2
+    lead, m = range(x.dim() - 7), x.dim() - 7
+    order = (0, 4, 1, 3, 2, 5, 6) if D == 128 else (4, 1, 0, 3, 2, 5, 6)
+    x = x.permute(*lead, *(m + k for k in order))
+    return (x[..., 0] | (x[..., 1] << 4)).flatten(-6)
+
+
+def _records(kc, ks, km, vc, vs, vm):
+    """Records of 16 tokens: codes (..., 16, D) and parameters (..., 16, groups) of keys and values."""
+    pairs = [torch.stack(p, -1).flatten(-3).view(torch.uint8) for p in ((ks, km), (vs, vm))]
+    return torch.cat([_key_bytes(kc), _value_bytes(vc), *pairs], -1)
+
+
+def _scatter(data, pieces, where):
+    """Write whole records: pieces (n, n_kv, records per block, bytes) into blocks `where` of data."""
+    data[where] = pieces
+
+
+def _fill(gen, case, blocks_in_use, total_blocks):
+    """A cache whose blocks in use hold quantised activations, and the codes behind it."""
+    n_kv, D, P = case["n_kv"], case["dim"], case["block"]
+    dtype = DTYPES[case["dtype"]]
+    size = 16 * D + 128 * (D // case["group"])
+    data = torch.randint(0, 256, (total_blocks, n_kv, P // 16, size), dtype=torch.uint8, generator=gen, device="cuda")
+    kinds = []
+    step = max(1, (1 << 27) // (n_kv * P * D))
+    where = blocks_in_use.long()
+    for at in range(0, where.numel(), step):
+        some = where[at:at + step]
+        parts = []
+        for _ in range(2):
+            c, s, m = _quantise(_heads(gen, (some.numel(), n_kv, P // 16, 16, D), dtype), case["group"])
+            parts += [c, s, m]
+        _scatter(data, _records(*parts), some)
+        kinds.append(parts)
+    return data, kinds
+
+
+def _make(case, seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    rng = random.Random(seed)
+    if case["op"] == "plan":
+        ctx, new = _lens(case)
+        P = case["block"]
+        have = [_blocks(c, P) for c in ctx]
+        need = sum(_blocks(c + n, P) for c, n in zip(ctx, new)) - sum(have)
+        spare = max(0, need - case["short"]) if case["short"] else need + 10
+        ids = list(range(sum(have) + spare))
+        rng.shuffle(ids)
+        width = max(_blocks(c + n, P) for c, n in zip(ctx, new)) + 3
+        table, at = [], 0
+        for h in have:
+            table.append(ids[at:at + h] + [-1] * (width - h))
+            at += h
+        free = ids[at:] + [-1] * 7
+        return dict(case=dict(case), context_lens=_int32(ctx), new_lens=_int32(new), block_tables=_int32(table),
+                    free_blocks=_int32(free), n_free=_int32([spare]), n_tokens=sum(new) + case["lens"] % 2 * 3), None
+    dtype = DTYPES[case["dtype"]]
+    if case["op"] == "store":
+        B, S, n_kv, D, P = case["batch"], case["tokens"], case["n_kv"], case["dim"], case["block"]
+        total = B * (_blocks(S, P) + 1)
+        size = 16 * D + 128 * (D // case["group"])
+        data = torch.randint(0, 256, (total, n_kv, P // 16, size), dtype=torch.uint8, generator=gen, device="cuda")
+        k, v = (_heads(gen, (B, n_kv, S, D), dtype) for _ in range(2))
+        blocks = torch.randperm(total, generator=gen, device="cuda").view(B, -1)
+        first = torch.tensor([rng.randrange(P) for _ in range(B)], device="cuda")
+        at = first[:, None] + torch.arange(S, device="cuda")  # each sequence starts inside its first block
+        slots = (blocks.gather(1, at // P) * P + at % P).int().flatten()
+        if S > 8:
+            slots[rng.randrange(B * S)] = -1  # a token that is padding
+        return dict(case=dict(case), data=data, k=k, v=v, slots=slots), None
+    ctx, new = _lens(case)
+    P, D = case["block"], case["dim"]
+    counts = [_blocks(c + n, P) for c, n in zip(ctx, new)]
+    total = sum(counts) + 5
+    ids = torch.randperm(total, generator=gen, device="cuda").int()
+    table = torch.full((len(ctx), max(counts) + 1), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(counts):
+        table[r, :n] = ids[at:at + n]
+        at += n
+    data, kinds = _fill(gen, case, ids[:at], total)
+    q = _heads(gen, (sum(new), case["n_q"], D), dtype)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    state = dict(case=dict(case), data=data, block_tables=table, seq_lens=_int32([c + n for c, n in zip(ctx, new)]),
+                 q=q, query_start=_int32(starts), max_new=max(new))
+    return state, (kinds, counts, ctx, new)
+
+
+def prepare(case, seed):
+    return _make(case, seed)[0]
+
+
+# ------------------------------------------------------------------ plain forms
+def _plain_plan(s):
+    ctx, new, table, P = s["context_lens"].long(), s["new_lens"].long(), s["block_tables"], s["case"]["block"]
+    width, n_free = table.shape[1], s["n_free"].long()
+    ends = new.cumsum(0)
+    have, want = (ctx + P - 1) // P, (ctx + new + P - 1) // P
+    fits = (want <= width) & (ends <= s["n_tokens"])
+    need = torch.where(fits, want - have, 0)
+    upto = need.cumsum(0)
+    granted = fits & ((need == 0) | (upto <= n_free))
+    need = torch.where(granted, need, 0)
+    before = upto - need
+    col = torch.arange(width, device=ctx.device)
+    nth = before[:, None] + col - have[:, None]
+    fresh = (col >= have[:, None]) & (col < (have + need)[:, None])
+    from_list = s["free_blocks"].long()[(n_free - 1 - nth).clamp(0, s["free_blocks"].numel() - 1)]
+    table.copy_(torch.where(fresh, from_list, table.long()))
+    token = torch.arange(s["n_tokens"], device=ctx.device)
+    owner = torch.searchsorted(ends, token, right=True).clamp(max=len(ctx) - 1)
+    inside = token < ends[-1]
+    position = torch.where(inside, ctx[owner] + token - (ends - new)[owner], 0)
+    block = table.long()[owner, (position // P).clamp(max=width - 1)]
+    slot = torch.where(inside & granted[owner], block * P + position % P, -1)
+    start = torch.cat([ends.new_zeros(1), ends]).clamp(max=s["n_tokens"])
+    return dict(block_tables=table, query_start=start.int(), positions=position.int(), slots=slot.int(),
+                seq_lens=torch.where(granted, ctx + new, 0).int(), n_free=(n_free - need.sum()).int(),
+                refused=(~granted).sum().int().view(1))
+
+
+def _codes(records, D):
+    """Codes of the keys and the values, (..., 16, D) each, from records (..., bytes)."""
+    lead = records.shape[:-1]
+    nib = torch.stack([records[..., :16 * D] & 15, records[..., :16 * D] >> 4], -1)  # (..., bytes, j % 2)
+    m = len(lead)
+    k = nib[..., :8 * D, :].reshape(*lead, 16, 4, D // 32, 2, 2, 2)  # t | c, i, b, j / 2, j % 2
+    k = k.permute(*range(m + 1), m + 2, m + 1, m + 4, m + 5, m + 3).reshape(*lead, 16, D)
+    if D == 128:
+        v = nib[..., 8 * D:, :].reshape(*lead, 2, 8, 4, D // 32, 2, 2, 2)  # h, g, c, i, b, j / 2, j % 2
+        v = v.permute(*range(m), m, m + 2, m + 4, m + 3, m + 1, m + 5, m + 6)
+    else:
+        v = nib[..., 8 * D:, :].reshape(*lead, 8, 4, 2, D // 32, 2, 2, 2)  # g, c, h, i, b, j / 2, j % 2
+        v = v.permute(*range(m), m + 2, m + 1, m + 4, m + 3, m, m + 5, m + 6)
+    return k, v.reshape(*lead, 16, D)
+
+
+def _values(records, D, dtype):
+    """What records (..., bytes) stand for: keys and values (..., 16, D) in 32 bits."""
+    k, v = _codes(records, D)
+    pair = records[..., 16 * D:].contiguous().view(dtype).float().unflatten(-1, (2, 16, -1, 2))
+    out = []
+    for x, p in ((k, pair[..., 0, :, :, :]), (v, pair[..., 1, :, :, :])):
+        g = x.float().unflatten(-1, (p.shape[-2], -1))
+        out.append((g * p[..., 0, None] + p[..., 1, None]).flatten(-2))
+    return out
+
+
+def _plain_store(s):
+    c = s["case"]
+    n_kv, D, P, dtype = c["n_kv"], c["dim"], c["block"], DTYPES[c["dtype"]]
+    keep = s["slots"] >= 0
+    slot = s["slots"][keep].long()
+    block, record, row = slot // P, slot % P // 16, slot % 16
+    k, v = (x.transpose(1, 2).reshape(-1, n_kv, D)[keep] for x in (s["k"], s["v"]))
+    (kc, ks, km), (vc, vs, vm) = _quantise(k, c["group"]), _quantise(v, c["group"])
+    # each token's bytes: a record that holds the token in its row and nothing in the other rows
+    rows = torch.arange(16, device=slot.device)
+    mine = (rows == row[:, None])[:, None, :, None]  # token, head, row, dim
+
+    def placed(x):
+        return torch.where(mine, x.unsqueeze(2), torch.zeros((), dtype=x.dtype, device=x.device))
+
+    piece = _records(*(placed(x) for x in (kc, ks, km, vc, vs, vm)))
+    ones = torch.full_like(kc, 15)
+    full = torch.full_like(ks.view(torch.int16), -1).view(dtype)
+    mask = _records(*(placed(x) for x in (ones, full, full, ones, full, full)))
+    # records shared by several tokens: their pieces do not overlap, so they add up
+    key = block * (P // 16) + record
+    some, which = torch.unique(key, return_inverse=True)
+
+    def joined(x):
+        return torch.zeros(some.numel(), *x.shape[1:], dtype=torch.int32, device=x.device).index_add_(
+            0, which, x.to(torch.int32)).to(torch.uint8)
+
+    where = (some // (P // 16), slice(None), some % (P // 16))
+    s["data"][where] = (s["data"][where] & ~joined(mask)) | joined(piece)
+    token = torch.arange(slot.numel(), device=slot.device)
+    got = s["data"][block, :, record]  # token, head, bytes
+    out = []
+    for x in _values(got, D, dtype):
+        whole = torch.zeros(s["slots"].numel(), n_kv, D, dtype=dtype, device=x.device)
+        whole[keep] = x[token, :, row].to(dtype)
+        out.append(whole)
+    return dict(k=out[0], v=out[1])
+
+
+def _plain_attend(s):
+    c = s["case"]
+    R, n_q, n_kv, D, P = c["requests"], c["n_q"], c["n_kv"], c["dim"], c["block"]
+    total, start = s["seq_lens"].long(), s["query_start"].long()
+    new = start[1:] - start[:-1]
+    blocks = s["block_tables"].long().clamp(min=0)
+    k, v = (x.reshape(R, n_kv, 1, -1, D)
+            for x in _values(s["data"][blocks].transpose(1, 2).flatten(2, 3), D, DTYPES[c["dtype"]]))
+    j = torch.arange(s["max_new"], device=total.device)
+    live = j < new[:, None]  # request, query
+    token = (start[:-1, None] + j).clamp(max=s["q"].shape[0] - 1)
+    q = s["q"].float()[token].transpose(1, 2).reshape(R, n_kv, n_q // n_kv, -1, D)
+    key = torch.arange(k.shape[3], device=total.device)
+    position = (total - new)[:, None] + j
+    seen = (key <= position[..., None]) & live[..., None]
+    if c["window"]:
+        seen &= key > position[..., None] - c["window"]
+    seen = seen[:, None, None]
+    score = (q @ k.transpose(-1, -2)).mul_(1 / math.sqrt(D)).masked_fill_(~seen, -math.inf)
+    top = score.amax(-1, keepdim=True).clamp(min=-1e30)
+    score.sub_(top).exp_()
+    v = v.masked_fill((key >= total[:, None])[:, None, None, :, None], 0.0)
+    out = (score @ v) / score.sum(-1, keepdim=True).clamp(min=1e-30)
+    out = out.reshape(R, n_q, -1, D).transpose(1, 2)
+    return out[live].to(s["q"].dtype)
+
+
+# ------------------------------------------------------------------ the package's calls
+@functools.lru_cache(maxsize=None)
+def _package():
+    sys.path.insert(0, os.path.join(os.getcwd(), "fused-triton-rmsnorm-residual-qkv_b200"))
+    import triton_fused_rmsnorm_qkv
+
+    return triton_fused_rmsnorm_qkv
+
+
+def _cache(ops, s):
+    c = s["case"]
+    if "cache" not in s:
+        s["cache"] = ops.KV4Cache(s["data"], head_dim=c["dim"], block_size=c["block"], group_size=c["group"],
+                                  dtype=DTYPES[c["dtype"]])
+    return s["cache"]
+
+
+def run(state):
+    s, c = state, state["case"]
+    if not own:
+        return {"plan": _plain_plan, "store": _plain_store, "attend": _plain_attend}[c["op"]](s)
+    ops = _package()
+    if c["op"] == "plan":
+        p = ops.kv4_plan(s["context_lens"], s["new_lens"], s["block_tables"], s["free_blocks"], s["n_free"],
+                         block_size=c["block"], n_tokens=s["n_tokens"])
+        return dict(block_tables=s["block_tables"], query_start=p.query_start, positions=p.positions, slots=p.slots,
+                    seq_lens=p.seq_lens, n_free=p.n_free, refused=p.refused)
+    if c["op"] == "store":
+        cache = _cache(ops, s)
+        ops.kv4_append(cache, s["k"], s["v"], s["slots"])
+        k, v = ops.kv4_gather(cache, s["slots"])
+        return dict(k=k, v=v)
+    return ops.kv4_attention(s["q"], _cache(ops, s), s["block_tables"], s["seq_lens"], s["query_start"],
+                             max_query_len=s["max_new"], window=c["window"] or None)
+
+
+# ------------------------------------------------------------------ 64 bits
+def exact(case, seed):
+    """The definition in 64 bits: a cached number is scale * code + minimum, with the scale and the
+    minimum as the cache holds them; attention is a softmax over the tokens that a query sees."""
+    s, made = _make(case, seed)
+    if case["op"] == "plan":
+        return None
+    if case["op"] == "store":
+        out = {}
+        for name in ("k", "v"):
+            x = s[name].double().transpose(1, 2).reshape(-1, case["n_kv"], case["dim"])
+            g = x.reshape(*x.shape[:-1], -1, case["group"])
+            low = g.min(-1, keepdim=True).values
+            scale = ((g.max(-1, keepdim=True).values - low).float() / 15).to(s[name].dtype).double()
+            code = torch.clamp(torch.round((g - low) / scale), 0, 15)
+            whole = torch.where(scale > 0, scale * code, 0.0) + low
+            whole = whole.reshape(x.shape)
+            whole[s["slots"] < 0] = 0
+            out[name] = whole
+        return out
+    kinds, counts, ctx, new = made
+    D, P, n_kv = case["dim"], case["block"], case["n_kv"]
+    dense = []
+    for at in (0, 3):
+        parts = []
+        for p in kinds:
+            code, scale, low = (x.double() for x in p[at:at + 3])
+            code = code.reshape(*code.shape[:-1], -1, case["group"])
+            parts.append((code * scale[..., None] + low[..., None]).reshape(code.shape[0], n_kv, P, D))
+        dense.append(torch.cat(parts))
+    out, block, token = [], 0, 0
+    for r, n in enumerate(counts):
+        total = ctx[r] + new[r]
+        k, v = (x[block:block + n].transpose(0, 1).reshape(n_kv, n * P, D)[:, :total] for x in dense)
+        block += n
+        q = s["q"][token:token + new[r]].double().transpose(0, 1)
+        token += new[r]
+        pos = ctx[r] + torch.arange(new[r], device=q.device)[:, None]
+        key = torch.arange(total, device=q.device)[None]
+        hidden = key > pos
+        if case["window"]:
+            hidden = hidden | (key <= pos - case["window"])
+        heads = []
+        for h in range(case["n_q"]):
+            g = h // (case["n_q"] // n_kv)
+            logits = (q[h] @ k[g].T) * D ** -0.5
+            logits[hidden] = -math.inf
+            heads.append(torch.softmax(logits, -1) @ v[g])
+        out.append(torch.stack(heads, 1))
+    return torch.cat(out)
