@@ -12,7 +12,7 @@ RMSNorm + Q/K/V projection with the rotary embedding:
 The cache's bytes.  A block of P tokens of one KV head is P / 16 records of 16 tokens; a record
 holds the keys' codes, the values' codes, then one (scale, minimum) pair of 16-bit numbers per
 token and group of dims, for the keys and for the values: 16 D + 128 D / group bytes.  A code c
-stands for scale * c + minimum.
+stands for scale * c + minimum; the scale is (maximum - minimum) * float32(1 / 15), rounded to 16 bits.
   keys    token t, dim d = 32 i + 8 c + 2 j + b sits in byte t D/2 + c D/8 + 4 i + 2 b + j / 2
           (low half of the byte for even j)
   values  token t = 8 h + 2 c + b, dim d = 32 i + 4 g + j sits in the 16-bit word
@@ -170,7 +170,7 @@ def _quantise(x, group):
     """(codes, scale, minimum) of rows x (..., D): codes 0..15, scale and minimum in x's type."""
     g = x.float().unflatten(-1, (-1, group))
     low, high = g.amin(-1), g.amax(-1)
-    scale, low = ((high - low) / 15).to(x.dtype), low.to(x.dtype)
+    scale, low = ((high - low) * (1 / 15)).to(x.dtype), low.to(x.dtype)
     s = scale.float().unsqueeze(-1)
     code = torch.where(s > 0, ((g - low.float().unsqueeze(-1)) / s).round().clamp(0, 15), 0.0)
     return code.to(torch.uint8).flatten(-2), scale, low
@@ -455,7 +455,7 @@ def exact(case, seed):
             x = s[name].double().transpose(1, 2).reshape(-1, case["n_kv"], case["dim"])
             g = x.reshape(*x.shape[:-1], -1, case["group"])
             low = g.min(-1, keepdim=True).values
-            scale = ((g.max(-1, keepdim=True).values - low).float() / 15).to(s[name].dtype).double()
+            scale = ((g.max(-1, keepdim=True).values - low).float() * (1 / 15)).to(s[name].dtype).double()
             code = torch.clamp(torch.round((g - low) / scale), 0, 15)
             whole = torch.where(scale > 0, scale * code, 0.0) + low
             whole = whole.reshape(x.shape)
