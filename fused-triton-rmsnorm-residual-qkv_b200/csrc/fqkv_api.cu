@@ -267,6 +267,17 @@ int validate(const Problem& p) {
 
 }  // namespace
 
+// The same reporting and device query for the library's other entry points (fqkv_kv4_api.cu).
+int api_fail(int code, const char* msg) { return fail(code, "%s", msg); }
+int api_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int api_sm100(int* sms) {
+  DeviceInfo d;
+  if (int rc = device_info(&d)) return rc;
+  if (d.major != 10) return fail(FQKV_ERR_DEVICE, "compute capability %d.%d is not sm_100", d.major, d.minor);
+  *sms = d.sms;
+  return 0;
+}
+
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel, device) and size:
 // the attribute only has to cover the largest request seen.
 cudaError_t ensure_smem_attr(const void* func, size_t bytes) {

@@ -5,7 +5,9 @@ Import-compatible with the reference package ``triton_fused_rmsnorm_qkv``
 ``fused_add_rmsnorm_matmul`` (returns the updated residual as well) and
 ``qkv_rope_split`` (head-major Q/K/V with the rotary embedding, one launch) and
 ``fused_add_rmsnorm_matmul_fp8w`` (e4m3 weights with a scale per row, decode sizes) and
-``schedule_info`` (the schedule an automatic call of a shape runs).  The GPU entry
+``schedule_info`` (the schedule an automatic call of a shape runs), and the paged 4-bit
+key/value cache behind the projection (``kv4_plan``, ``kv4_append``, ``kv4_gather``,
+``kv4_attention``).  The GPU entry
 points run sm_100a CUDA kernels from ``libfqkv.so``; they raise if that library is
 missing instead of falling back to anything else.
 """
@@ -24,6 +26,7 @@ from .kernel import (
     quantize_weight_e4m3,
     schedule_info,
 )
+from .kv4 import KV4Cache, KV4Plan, kv4_append, kv4_attention, kv4_cache, kv4_gather, kv4_plan
 
 __all__ = [
     "rmsnorm_residual_qkv",
@@ -39,4 +42,11 @@ __all__ = [
     "fused_add_rmsnorm_matmul_fp8w",
     "quantize_weight_e4m3",
     "schedule_info",
+    "KV4Cache",
+    "KV4Plan",
+    "kv4_cache",
+    "kv4_plan",
+    "kv4_append",
+    "kv4_gather",
+    "kv4_attention",
 ]

@@ -21,6 +21,7 @@ FLAG_PDL, FLAG_STATIC_WEIGHTS, FLAG_TEST_WITHHOLD = 1, 2, 4
 ERR_NULL, ERR_SHAPE, ERR_DTYPE, ERR_ALIGN, ERR_WORKSPACE, ERR_SCHEDULE, ERR_DEVICE, ERR_DEVICE_TIMEOUT, ERR_ALIAS = (
     1, 2, 3, 4, 5, 6, 7, 8, 9)
 STATUS_WAIT_TIMEOUT = 1
+STATUS_BAD_INDEX = 2
 
 SCHEDULE_NAMES = {SCHED_SIMT: "simt", SCHED_DECODE: "decode", SCHED_SPLIT: "split", SCHED_PREFILL: "prefill",
                   SCHED_GRID: "grid"}
@@ -43,6 +44,12 @@ EXPORTED_SYMBOLS = (
     "fqkv_stream_capture_id",
     "fqkv_test_set_wait_limit_ns",
     "fqkv_version",
+    "fqkv_kv4_record_bytes",
+    "fqkv_kv4_plan",
+    "fqkv_kv4_append",
+    "fqkv_kv4_gather",
+    "fqkv_kv4_attention",
+    "fqkv_kv4_workspace_bytes",
 )
 
 
@@ -57,7 +64,17 @@ class ScheduleInfo(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class KV4CacheDesc(ctypes.Structure):
+    """``fqkv_kv4_cache``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("n_blocks", ctypes.c_int64), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("group_size", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 _lib = None
+# The cache's calls by name (load fills it): the CPython module's where it is built, ctypes' otherwise.
+kv4: dict = {}
 # CPython fast path for fqkv_launch (csrc/fqkv_pycall.c, built by build.py); ctypes otherwise.
 try:
     from . import _fqkv_pycall as _pycall
@@ -102,6 +119,23 @@ def load() -> ctypes.CDLL:
     lib.fqkv_launch_rope.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, vp,
                                      i64, i32, i32, i32, f32, i32, i32, vp]
     lib.fqkv_launch_rope.restype = i32
+    lib.fqkv_kv4_record_bytes.argtypes = [i64, i64]
+    lib.fqkv_kv4_record_bytes.restype = i64
+    lib.fqkv_kv4_workspace_bytes.argtypes = [i64, i64, i64, i64]
+    lib.fqkv_kv4_workspace_bytes.restype = i64
+    lib.fqkv_kv4_plan.argtypes = [vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.fqkv_kv4_append.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, vp, i64, vp]
+    lib.fqkv_kv4_gather.argtypes = [vp, vp, i64, vp, vp, i64, vp]
+    lib.fqkv_kv4_attention.argtypes = [vp, vp, i64, i64, i64, i64, vp, i64, i64, i64, i64, vp, i64, i64, vp, i64, f32,
+                                       vp, i64, vp, i64, i64, vp]
+    names = ("plan", "append", "gather", "attention")
+    for name in names:
+        getattr(lib, f"fqkv_kv4_{name}").restype = i32
+    if _pycall is not None and hasattr(_pycall, "set_kv4"):
+        _pycall.set_kv4(*(ctypes.cast(getattr(lib, f"fqkv_kv4_{name}"), ctypes.c_void_p).value for name in names))
+        kv4.update({name: getattr(_pycall, f"kv4_{name}") for name in names})
+    else:
+        kv4.update({name: getattr(lib, f"fqkv_kv4_{name}") for name in names})
     if _pycall is not None:
         _pycall.set_launch(ctypes.cast(lib.fqkv_launch, ctypes.c_void_p).value)
     _lib = lib

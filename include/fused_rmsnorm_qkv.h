@@ -96,6 +96,8 @@ extern "C" {
 /* Bits of the device status word. */
 #define FQKV_STATUS_OK            0
 #define FQKV_STATUS_WAIT_TIMEOUT  1  /* an mbarrier wait gave up after its iteration limit */
+#define FQKV_STATUS_BAD_INDEX     2  /* a block, slot, length or token start read from device memory was
+                                        out of range; the access it would have caused was not made */
 
 /* Description of the schedule the library would run (replaces the Triton
  * autotune record returned by get_autotune_best_config, kernel.py:558-572). */
@@ -242,7 +244,107 @@ FQKV_API int fqkv_rope_split(const void* qkv, int64_t ldq, const void* cos, cons
                 int64_t cos_batch, void* q, void* k, void* v, int64_t B, int64_t S,
                 int n_q_heads, int n_kv_heads, int head_dim, int dtype, void* stream);
 
-/* ABI version (major * 100 + minor): 102 adds FQKV_SCHED_GRID. */
+/* ------------------------------------------------------------------------------------
+ * Paged 4-bit key/value cache: block tables and slots planned on the GPU, rotated keys and
+ * values quantised into their slots, and causal attention over the 4-bit codes.  No
+ * counterpart in the reference (its integration uses transformers' 16-bit cache).
+ *
+ * The cache is one array of n_blocks * n_kv_heads * (block_size / 16) records.  Record
+ * (block b, head h, i) holds tokens 16 i .. 16 i + 15 of the block for that KV head:
+ *   8 D bytes       4-bit codes of the keys
+ *   8 D bytes       4-bit codes of the values
+ *   64 NG bytes     the keys' parameters: per token and group {scale, minimum}, 16-bit each
+ *   64 NG bytes     the values' parameters, the same way
+ * with D = head_dim and NG = D / group_size.  Code c of token t, dim d stands for
+ *   scale[t, d / group_size] * c + minimum[t, d / group_size].
+ * Byte places of the codes (low half of the byte for even j):
+ *   keys    t * D/2 + c * D/8 + 4 i + 2 b + j / 2            d = 32 i + 8 c + 2 j + b
+ *   values  16-bit word (h, g, c, i, b) for D = 128, (g, c, h, i, b) for D = 64, bits 4 j;
+ *                                      t = 8 h + 2 c + b,    d = 32 i + 4 g + j
+ * so that a warp's 16-byte loads are the operand fragments of a tensor-core product.
+ * A slot is block * block_size + the token's place in the block.
+ * ------------------------------------------------------------------------------------ */
+typedef struct fqkv_kv4_cache {
+  void* data;          /* 128-byte aligned                                                */
+  int64_t n_blocks;
+  int32_t n_kv_heads;
+  int32_t head_dim;    /* 64 or 128                                                       */
+  int32_t block_size;  /* tokens per block, a multiple of 16                              */
+  int32_t group_size;  /* 32, 64 or 128 dims share a scale; divides head_dim              */
+  int32_t dtype;       /* FQKV_F16 / FQKV_BF16: keys, values, queries and parameters      */
+  int32_t reserved;    /* 0                                                               */
+} fqkv_kv4_cache;
+
+/* Bytes of one record (16 D + 128 D / group_size), or 0 for an unsupported pair. */
+FQKV_API int64_t fqkv_kv4_record_bytes(int64_t head_dim, int64_t group_size);
+
+/*
+ * Block tables, token positions and slots of a batch, from the requests' lengths.
+ *   context_lens, new_lens [R]  tokens cached before this step, tokens this step adds
+ *   block_tables [R, width] (row stride table_stride): the first ceil(context / block_size)
+ *                entries of a row are read, the entries of newly taken blocks are written
+ *   free_blocks  [free_capacity], n_free [1]: a stack whose first n_free entries are free;
+ *                blocks are taken from its end, request by request in order (neither is written)
+ * A request is granted when its blocks fit the table's width, its tokens end within n_tokens,
+ * and it needs no block or the blocks needed up to and including it are at most n_free.  A
+ * request that is not granted takes no blocks, has seq_lens 0 and slots -1, and is counted.
+ *   query_start [R + 1]  first token of each request (clipped to n_tokens)
+ *   positions, slots [n_tokens]  0 and -1 past the last request's tokens
+ *   seq_lens [R]  context + new, or 0;  n_free_out [1];  refused [1]
+ * All int32.  A negative length counts as 0 tokens and is refused.
+ */
+FQKV_API int fqkv_kv4_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t n_requests,
+                int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                const int32_t* free_blocks, int64_t free_capacity, const int32_t* n_free,
+                int64_t block_size, int64_t n_tokens, int32_t* query_start, int32_t* positions,
+                int32_t* slots, int32_t* seq_lens, int32_t* n_free_out, int32_t* refused,
+                int64_t flags, void* stream);
+
+/*
+ * Quantise keys and values into their slots.
+ *   k, v  token (b, s), head h at b * stride_b + s * stride_s + h * stride_h (elements; D
+ *         contiguous, 16-byte aligned), n_batch * n_seq tokens
+ *   slots [n_batch * n_seq]  distinct; negative: the token is skipped; past the cache: skipped
+ *         and FQKV_STATUS_BAD_INDEX
+ * Per token, head and group, in fp32: minimum = min x, scale = dtype((max x - min x) * (1/15)),
+ * code = clamp(rint((x - minimum) / scale), 0, 15) (0 where scale is 0).  A head row with a
+ * NaN or an infinity (or a scale that overflows) is stored as NaN parameters.
+ */
+FQKV_API int fqkv_kv4_append(const fqkv_kv4_cache* cache, const void* k, const void* v,
+                int64_t n_batch, int64_t n_seq, int64_t k_stride_b, int64_t k_stride_s, int64_t k_stride_h,
+                int64_t v_stride_b, int64_t v_stride_s, int64_t v_stride_h, const int32_t* slots,
+                int64_t flags, void* stream);
+
+/* What slots hold, as numbers: k, v [n_tokens, n_kv_heads, head_dim] in the cache's dtype
+ * (scale * code + minimum in fp32, rounded once); zeros for a negative slot. */
+FQKV_API int fqkv_kv4_gather(const fqkv_kv4_cache* cache, const int32_t* slots, int64_t n_tokens,
+                void* k, void* v, int64_t flags, void* stream);
+
+/*
+ * Causal attention of the batch's new tokens over the cache (their own keys and values
+ * already appended).  Request r has n = query_start[r + 1] - query_start[r] queries (n_seq
+ * each when query_start is NULL); its query j sees tokens t <= p and, with window > 0,
+ * t > p - window, where p = seq_lens[r] - n + j.  A query that sees nothing gives zeros.
+ *   q    request r, query j, head h at r * q_stride_r + j * q_stride_t + h * q_stride_h, or,
+ *        with query_start, token query_start[r] + j in the place of both; 16-byte aligned rows
+ *   out  [n_tokens, n_q_heads, head_dim] in the cache's dtype, row stride out_stride_t
+ *   scale  multiplies the scores; n_q_heads / n_kv_heads query heads share a KV head
+ *   max_query_len  an upper bound of n: a hint that chooses the kernel, any value is correct
+ *   workspace  fqkv_kv4_workspace_bytes(...) bytes, 256-byte aligned.  Its first 4096 bytes
+ *        (arrival counters) are zero before the first launch that uses it and every completed
+ *        launch leaves them zero; launches that share it must not overlap on the GPU.
+ */
+FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const void* q, int64_t q_stride_r,
+                int64_t q_stride_t, int64_t q_stride_h, int64_t n_q_heads, const int32_t* query_start,
+                int64_t n_tokens, int64_t n_seq, int64_t n_requests, int64_t max_query_len,
+                const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                const int32_t* seq_lens, int64_t window, float scale, void* out, int64_t out_stride_t,
+                void* workspace, int64_t workspace_bytes, int64_t flags, void* stream);
+FQKV_API int64_t fqkv_kv4_workspace_bytes(int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                int64_t max_query_len);
+
+/* ABI version (major * 100 + minor): 102 adds FQKV_SCHED_GRID (and, beside it, the fqkv_kv4_*
+ * entry points, which a caller finds by name). */
 FQKV_API int fqkv_version(void);
 
 #ifdef __cplusplus
