@@ -11,6 +11,7 @@ namespace fqkv {
 constexpr int kKv4Rec = 16;           // tokens per record
 constexpr int kKv4CounterBytes = 4096;  // arrival counters at the head of the attention workspace
 constexpr int kKv4MaxGrid = 320;      // CTAs of the split attention kernel, at most
+constexpr int kKv4PromptMaxGrid = 160;  // and of the prompt kernel
 
 // A record's byte offsets for head_dim D and NG groups: keys at 0, values at 8 D, the keys'
 // parameters at 16 D, the values' at 16 D + 64 NG.
@@ -76,6 +77,9 @@ cudaError_t launch_kv4_gather(const Kv4GatherParams& p, bool bf16, bool pdl, cud
 // Rows per item (8 or 16) by the row count hint.
 cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int row_blocks8, int sms, bool bf16, bool pdl,
                                   cudaStream_t stream);
+
+cudaError_t launch_kv4_attn_prompt(const Kv4AttnParams& p, int sms, bool bf16, bool pdl, cudaStream_t stream);
+int64_t kv4_prompt_partial_bytes(int D);
 
 template <typename... KArgs, typename... Args>
 cudaError_t kv4_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t stream,

@@ -1,6 +1,7 @@
 // fqkv_kv4_api.cu -- the extern "C" boundary of the paged 4-bit key/value cache
 // (include/fused_rmsnorm_qkv.h).  Arguments are checked before any CUDA call; nothing is
 // allocated or synchronised.
+#include <cmath>
 #include <cstdint>
 
 #include "fqkv_kv4.cuh"
@@ -9,6 +10,8 @@ using namespace fqkv;
 
 namespace {
 
+// More query rows (heads that share a KV head, times queries) than this go to the prompt kernel.
+constexpr int64_t kPromptRows = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -40,10 +43,14 @@ int check_flags(int64_t flags) {
 
 int done(cudaError_t e, const char* what) { return e == cudaSuccess ? 0 : api_cuda_fail(e, what); }
 
-// Rows of an item of the split kernel, in eights.
-int row_blocks8(int64_t G, int64_t max_query_len) { return G * max_query_len <= 8 ? 1 : 2; }
+// Rows of an item of the split kernel, in eights; 0: the prompt kernel.
+int row_blocks8(int64_t G, int64_t max_query_len) {
+  if (max_query_len > kPromptRows / G) return 0;
+  return G * max_query_len <= 8 ? 1 : 2;
+}
 
-int64_t split_workspace(int64_t head_dim, int rb8) {
+int64_t workspace_size(int64_t head_dim, int rb8) {
+  if (rb8 == 0) return kKv4CounterBytes + kv4_prompt_partial_bytes((int)head_dim);
   return kKv4CounterBytes + (int64_t)2 * kKv4MaxGrid * 8 * rb8 * (head_dim + 2) * 4;
 }
 
@@ -120,7 +127,7 @@ extern "C" FQKV_API int64_t fqkv_kv4_workspace_bytes(int64_t n_q_heads, int64_t 
   if (n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) ||
       max_query_len < 0)
     return -FQKV_ERR_SHAPE;
-  return split_workspace(head_dim, row_blocks8(n_q_heads / n_kv_heads, max_query_len));
+  return workspace_size(head_dim, row_blocks8(n_q_heads / n_kv_heads, max_query_len));
 }
 
 extern "C" FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const void* q, int64_t q_stride_r,
@@ -143,6 +150,8 @@ extern "C" FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const vo
       table_width > INT32_MAX / c.P)
     return api_fail(FQKV_ERR_SHAPE, "max_query_len and window must not be negative, table_stride at least table_width, "
                                     "and a table's tokens below 2^31");
+  if (!(fabsf(scale) > 0.0f && fabsf(scale) <= 1e30f))
+    return api_fail(FQKV_ERR_SHAPE, "scale must be finite and not zero");
   if (out_stride_t < n_q_heads * c.D) return api_fail(FQKV_ERR_SHAPE, "out_stride_t is smaller than a token's row");
   if (!aligned(q, 16) || ((q_stride_r | q_stride_t | q_stride_h) & 7) || !aligned(out, 16) || (out_stride_t & 7))
     return api_fail(FQKV_ERR_ALIGN, "q and out rows must be 16-byte aligned (strides multiples of 8 elements)");
@@ -175,7 +184,8 @@ extern "C" FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const vo
   p.counters = static_cast<int*>(workspace);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv4CounterBytes);
   const bool pdl = flags & FQKV_FLAG_PDL, bf16 = cache->dtype == FQKV_BF16;
-  return done(launch_kv4_attn_split(p, row_blocks8(p.G, max_query_len), sms, bf16, pdl,
-                                    static_cast<cudaStream_t>(stream)),
+  const int rb8 = row_blocks8(p.G, max_query_len);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return done(rb8 ? launch_kv4_attn_split(p, rb8, sms, bf16, pdl, st) : launch_kv4_attn_prompt(p, sms, bf16, pdl, st),
               "attention launch");
 }
