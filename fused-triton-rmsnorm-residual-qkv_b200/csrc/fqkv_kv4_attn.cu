@@ -27,16 +27,13 @@
 // takes a contiguous part of a piece with a ring of its own, filled by bulk copies of whole
 // records.  An item cut between CTAs is joined by the CTA that arrives last, which adds the
 // parts in the order of the CTAs, so the result does not depend on the arrival order.
-#include "fqkv_kv4.cuh"
+#include "fqkv_kv4_work.cuh"
 
 namespace fqkv {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;    // tokens per ring stage (two records)
 constexpr int kStages = 2;
-constexpr int kMinTiles = 8;  // a CTA gets at least one tile per warp before the work is cut finer
 
 // Untiled bulk copy global -> shared, counted on a local mbarrier.  Addresses and size are
 // multiples of 16 bytes.
@@ -52,63 +49,40 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles j and j + 4 of w (bits 4 j and 16 + 4 j) as a pair of 16-bit floats offset() + code.
-template <typename T>
-struct Nib;
-template <>
-struct Nib<__nv_bfloat16> {
-  static constexpr float kOffset = 128.0f;  // 0x4300: four mantissa bits of weight 1..8
-  static constexpr float kMinNormal = 1e-30f;
-  static constexpr uint32_t kCentre = 0x43084308u;  // 136 = offset + 8
-  template <int j>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    return ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
-  }
-  static __device__ __forceinline__ uint32_t centred(uint32_t x) {
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(kCentre));
-    return r;
-  }
-};
-template <>
-struct Nib<__half> {
-  static constexpr float kOffset = 64.0f;  // 0x5400: mantissa bits 4..7 have weight 1..8
-  static constexpr float kMinNormal = 6.2e-5f;
-  static constexpr uint32_t kCentre = 0x54805480u;  // 72 = offset + 8
-  template <int j>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    const uint32_t x = j == 0 ? w << 4 : w >> (4 * (j > 0 ? j - 1 : 0));
-    return (x & 0x00F000F0u) | 0x54005400u;
-  }
-  static __device__ __forceinline__ uint32_t centred(uint32_t x) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(kCentre));
-    return r;
-  }
-};
+// Eight codes of a word as four fp16 pairs (nibbles j and j + 4): 1024 + code for j = 0, 2, where
+// the four bits are the mantissa's lowest, 64 + code for j = 1, 3, where they are bits 4-7.
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t& p0, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
+  const uint32_t v = w >> 8;
+  p0 = (w & 0x000F000Fu) | 0x64006400u;
+  p1 = (w & 0x00F000F0u) | 0x54005400u;
+  p2 = (v & 0x000F000Fu) | 0x64006400u;
+  p3 = (v & 0x00F000F0u) | 0x54005400u;
+}
+constexpr uint32_t kCentreLow = 0x64086408u;   // 1032 = 1024 + 8
+constexpr uint32_t kCentreHigh = 0x54805480u;  // 72 = 64 + 8
+
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
 
 template <typename T>
 __device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
   lo = Elem<T>::to_f((uint16_t)w);
   hi = Elem<T>::to_f((uint16_t)(w >> 16));
+}
+template <>
+__device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xFFFF0000u);
 }
 
 // a / b by an approximate reciprocal and one step of refinement; exact where the quotient is a
@@ -118,6 +92,12 @@ __device__ __forceinline__ float quotient(float a, float b) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(b));
   const float q = a * r;
   return fmaf(fmaf(-q, b, a), r, q);
+}
+
+__device__ __forceinline__ float log2_approx(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 template <int N>
@@ -133,229 +113,210 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// One request as the kernel sees it: lengths clamped to what the tables and q hold.
-struct Request {
-  int start, n, len;  // first token, queries, keys
-};
-
-__device__ __forceinline__ Request load_request(const Kv4AttnParams& p, int r) {
-  Request q;
-  int64_t a, b;
-  if (p.query_start) {
-    a = p.query_start[r];
-    b = p.query_start[r + 1];
-  } else {
-    a = (int64_t)r * p.S;
-    b = a + p.S;
-  }
-  const int64_t a0 = a, b0 = b;
-  a = a < 0 ? 0 : a > p.T ? p.T : a;
-  b = b < a ? a : b > p.T ? p.T : b;
-  const int len0 = p.seq_lens[r];
-  const int64_t cap = (int64_t)p.width * p.c.P;
-  q.len = len0 < 0 ? 0 : len0 > cap ? (int)cap : len0;
-  q.start = (int)a;
-  q.n = (int)(b - a);
-  if (a != a0 || b != b0 || q.len != len0) record_status(FQKV_STATUS_BAD_INDEX);
-  return q;
-}
-
-// Row block rb of a request: query rows [rb * ROWS, ...) of n * G rows (row = j * G + head).
-template <int ROWS>
-__device__ __forceinline__ void block_tiles(const Kv4AttnParams& p, const Request& q, int rb, int& tile_lo,
-                                            int& n_tiles) {
-  const int j0 = rb * ROWS / p.G, j1 = min((rb * ROWS + ROWS - 1) / p.G, q.n - 1);
-  const int hi = max(0, min(q.len, q.len - q.n + j1 + 1));
-  const int lo = p.window > 0 ? max(0, q.len - q.n + j0 - p.window + 1) : 0;
-  tile_lo = lo / kTile;
-  n_tiles = max(1, (hi + kTile - 1) / kTile - tile_lo);
-}
-
-template <int ROWS>
-__device__ __forceinline__ long long request_tiles(const Kv4AttnParams& p, const Request& q) {
-  const int blocks = (q.n * p.G + ROWS - 1) / ROWS;
-  long long sum = 0;
-  for (int rb = 0; rb < blocks; ++rb) {
-    int lo, n;
-    block_tiles<ROWS>(p, q, rb, lo, n);
-    sum += n;
-  }
-  return sum * p.c.n_kv;
-}
-
+// Warps of a CTA: two CTAs of eight on an SM for eight rows, one of twelve for sixteen rows (170
+// registers a thread); seven where eight rings of the largest records leave no room.
 template <int D, int NG, int NT>
-constexpr int ring_bytes() {
-  return kWarps * kStages * 2 * kv4_record_bytes(D, NG);
+constexpr int warps() {
+  return NT == 2 ? (D == 128 && NG == 4 ? 11 : 12) : D == 128 && NG == 4 ? 7 : 8;
 }
-// Per-column maxima and sums of the warps, and half of the warps' outputs for the tree sum.
+template <int D, int NG>
+constexpr int ring_bytes() {
+  return kStages * 2 * kv4_record_bytes(D, NG);
+}
+// A warp's part of an item as floats: its outputs by column, padded by four floats so that the
+// float4 stores of a quarter-warp (four columns, two dim groups) meet eight different bank groups.
+template <int D, int NT>
+constexpr int part_floats() {
+  return 8 * NT * (D + 4);
+}
 template <int D, int NG, int NT>
 constexpr int smem_bytes() {
-  return ring_bytes<D, NG, NT>() + kWarps / 2 * 8 * NT * D * 4;
+  return warps<D, NG, NT>() * (ring_bytes<D, NG>() + part_floats<D, NT>() * 4);
 }
 
+// What the join needs to know of a warp's part of an item.
+struct PartInfo {
+  long long item;  // first tile of the item in the batch; -1: no part
+  int n_tiles, row0, start, n, head0;
+};
+
 template <typename T, int D, int NG, int NT>
-__global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
+    kv4_attn_split_kernel(const Kv4AttnParams p) {
+  constexpr int WARPS = warps<D, NG, NT>(), THREADS = WARPS * 32;
   constexpr int ROWS = 8 * NT;           // query rows of an item
   constexpr int REC = kv4_record_bytes(D, NG);
   constexpr int NW = D / 32;             // 32-dim blocks: words per lane and key row
   constexpr int WPG = NW / NG;           // words of one scale group
+  constexpr int PART = part_floats<D, NT>();
+  static_assert(PART * 4 <= ring_bytes<D, NG>(), "a part fits the ring");
+  using Work = Kv4Work<ROWS, kTile, THREADS, WARPS>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_bar[kWarps][kStages];
-  __shared__ long long s_scan[kWarps];
-  __shared__ long long s_found;
-  __shared__ int s_r, s_last;
-  __shared__ float s_max[kWarps][ROWS], s_sum[kWarps][ROWS];
+  __shared__ uint64_t s_bar[WARPS][kStages];
+  __shared__ typename Work::Shared s_work;
+  __shared__ Work s_item[WARPS], s_ahead[WARPS];  // each warp's item, and the item its copies have reached
+  __shared__ PartInfo s_info[WARPS][2];
+  __shared__ float s_max[WARPS][2][ROWS], s_sum[WARPS][2][ROWS];
+  __shared__ int s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  uint8_t* ring = smem + warp * kStages * 2 * REC;
-  float* s_out = reinterpret_cast<float*>(smem + ring_bytes<D, NG, NT>());
-  if (tid < kWarps * kStages) mbar_init(&s_bar[tid / kStages][tid % kStages], 1);
-  if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  __syncthreads();
+  uint8_t* ring = smem + warp * ring_bytes<D, NG>();
+  float* parts = reinterpret_cast<float*>(smem + WARPS * ring_bytes<D, NG>());
+  // Slot 0: a part that the warp finished before its run ended.  Slot 1: its last part, in the
+  // ring, which is idle by then.
+  const auto part_at = [&](int w, int slot) -> float* {
+    return slot ? reinterpret_cast<float*>(smem + w * ring_bytes<D, NG>()) : parts + w * PART;
+  };
+  if (tid < WARPS * kStages) {
+    mbar_init(&s_bar[tid / kStages][tid % kStages], 1);
+    fence_mbarrier_init_cluster();
+  }
   pdl_wait();
   pdl_launch_dependents();
-
-  // ---- total work, and this CTA's run of tiles [u0, u1)
-  long long mine = 0;
-  for (int r = tid; r < p.R; r += kThreads) mine += request_tiles<ROWS>(p, load_request(p, r));
-  long long total = mine;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-  if (lane == 0) s_scan[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += s_scan[w];
-  const long long ctas = max(1ll, min((long long)gridDim.x, total / kMinTiles));
-  const long long cta = blockIdx.x;
-  if (cta >= ctas || total == 0) return;
-  const long long u0 = cta * total / ctas, u1 = (cta + 1) * total / ctas;
-
-  // ---- the request that holds tile u0
-  long long base = 0;
-  for (int r0 = 0; r0 < p.R; r0 += kThreads) {
-    const int r = r0 + tid;
-    const long long n = r0 == 0 && p.R <= kThreads ? mine
-                        : r < p.R                  ? request_tiles<ROWS>(p, load_request(p, r))
-                                                   : 0;
-    long long v = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(~0u, v, o);
-      if (lane >= o) v += u;
-    }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = v;
-    __syncthreads();
-    long long before = base;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += s_scan[w];
-      base += s_scan[w];
-    }
-    if (before + v - n <= u0 && u0 < before + v) {
-      s_r = r;
-      s_found = before + v - n;
-    }
-    if (base > u0) break;
-  }
-  __syncthreads();
-
-  int r = s_r;
-  Request req = load_request(p, r);
-  int blocks = (req.n * p.G + ROWS - 1) / ROWS;
-  int kvh = 0, rb = 0, tile_lo = 0, n_tiles = 0;
-  long long item = s_found;  // first tile of the current item
   {
-    const long long per_head = request_tiles<ROWS>(p, req) / p.c.n_kv;
-    kvh = (int)((u0 - item) / per_head);
-    item += kvh * per_head;
-    for (;; ++rb) {
-      block_tiles<ROWS>(p, req, rb, tile_lo, n_tiles);
-      if (u0 < item + n_tiles) break;
-      item += n_tiles;
+    Work first;
+    if (!first.locate(p, s_work, gridDim.x, WARPS)) return;  // its barriers publish the mbarriers
+    if (lane == 0) {
+      s_item[warp] = s_ahead[warp] = first;
+      s_info[warp][0].item = s_info[warp][1].item = -1;
     }
+    __syncwarp();
   }
+  // The warp's items live in shared memory: a few loads now and then instead of registers that the
+  // inner loop needs.
+  const Work& w = s_item[warp];
+  const long long run_end = w.b;
 
-  uint32_t parity = 0;  // bit s: phase of ring stage s
-  for (long long u = u0; u < u1;) {
-    // ---- one piece: tiles [u, ue) of item (r, kvh, rb); this warp's part [wt, we) of its tiles
-    const long long ue = min(u1, item + n_tiles);
-    const int piece = (int)(ue - u);
-    const int wt = tile_lo + (int)(u - item) + (int)((long long)piece * warp / kWarps);
-    const int we = tile_lo + (int)(u - item) + (int)((long long)piece * (warp + 1) / kWarps);
-    const int pos0 = req.len - req.n;  // position of query 0
-
-    // Record addresses: lane L holds record 2 * wt_base + L of the warp's tiles, 16 tiles at a time.
-    const int* table = p.table + (int64_t)r * p.table_stride;
-    const int n_rec = (req.len + kKv4Rec - 1) / kKv4Rec;
-    const int rpb = p.c.P / kKv4Rec;
-    const auto address = [&](int rec) -> const uint8_t* {
-      if (rec >= n_rec) return nullptr;
-      const int nth = rec / rpb;
-      int block = table[nth];
-      if (block < 0 || block >= p.c.n_blocks) {
-        record_status(FQKV_STATUS_BAD_INDEX);
-        block = 0;
-      }
-      return p.c.data + (((int64_t)block * p.c.n_kv + kvh) * rpb + (rec - nth * rpb)) * REC;
-    };
-    const uint8_t* src = address(2 * wt + lane);
-    const uint8_t* src_next = address(2 * wt + 32 + lane);
-    int src_tile = wt;  // src covers tiles [src_tile, src_tile + 16)
-    const auto issue = [&](int tile, int stage) {
-      if (tile - src_tile >= 16) {
-        src = src_next;
-        src_tile += 16;
-        src_next = address(2 * (src_tile + 16) + lane);
-      }
-      const int k = lane - 2 * (tile - src_tile);  // 0, 1: the lanes that hold this tile's records
-      const bool mine_rec = (k == 0 || k == 1) && src != nullptr;
-      const uint32_t have = __popc(__ballot_sync(~0u, mine_rec));
-      if (lane == 0) mbar_arrive_expect_tx(&s_bar[warp][stage], have * REC);
+  // ---- copies: the warp's run of tiles, in order, across its items
+  const uint8_t *src = nullptr, *src_next = nullptr;  // records 2 src_tile + lane, and the 32 after them
+  int src_tile = 0, ahead_tile, ahead_end;  // next tile to copy, end of this item's part of the run
+  int stage_in = 0;
+  long long ahead = w.a;
+  const auto address = [&](int rec) {
+    const Work& x = s_ahead[warp];
+    return kv4_record(p, p.table + (int64_t)x.r * p.table_stride, rec, (x.req.len + kKv4Rec - 1) / kKv4Rec,
+                      p.c.P / kKv4Rec, x.kvh, REC);
+  };
+  const auto enter = [&]() {
+    const Work& x = s_ahead[warp];
+    ahead_tile = x.tile_lo + (int)(ahead - x.item);
+    ahead_end = x.tile_lo + (int)(min(run_end, x.item + x.n_tiles) - x.item);
+    src_tile = ahead_tile;
+    src = address(2 * ahead_tile + lane);
+    src_next = 2 * ahead_end > 2 * ahead_tile + 32 ? address(2 * ahead_tile + 32 + lane) : nullptr;
+  };
+  const auto copy_next = [&]() {
+    if (ahead >= run_end) return;
+    if (ahead_tile == ahead_end) {
+      Work x = s_ahead[warp];
       __syncwarp();
-      if (mine_rec) bulk_load(smem_u32(ring + (stage * 2 + k) * REC), src, REC, &s_bar[warp][stage]);
-    };
+      x.next(p);
+      if (lane == 0) s_ahead[warp] = x;
+      __syncwarp();
+      enter();
+    }
+    if (ahead_tile - src_tile >= 16) {
+      src = src_next;
+      src_tile += 16;
+      if (ahead_end > src_tile + 16) src_next = address(2 * (src_tile + 16) + lane);
+    }
+    const int left = (s_ahead[warp].req.len + kKv4Rec - 1) / kKv4Rec - 2 * ahead_tile;  // records from here on
+    if (lane == 0)
+      mbar_arrive_expect_tx(&s_bar[warp][stage_in], (uint32_t)(left >= 2 ? 2 : max(left, 0)) * REC);
+    __syncwarp();
+    const uint32_t k = (uint32_t)(lane - 2 * (ahead_tile - src_tile));  // 0, 1: the lanes of this tile's records
+    if (k < 2 && src) bulk_load(smem_u32(ring + (stage_in * 2 + k) * REC), src, REC, &s_bar[warp][stage_in]);
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    ++ahead_tile;
+    ++ahead;
+  };
+  if (ahead < run_end) enter();
 #pragma unroll
-    for (int s = 0; s < kStages; ++s)
-      if (wt + s < we) issue(wt + s, s);
+  for (int s = 0; s < kStages; ++s) copy_next();
 
-    // ---- queries: this lane's fragments (row g of each 8) and the sums of its columns' rows
+  int stage = 0;
+  uint32_t parity = 0;  // bit s: phase of ring stage s
+  for (long long u = w.a; u < run_end;) {
+    // ---- a piece: tiles [u, ue) of item w
+    const long long ue = min(run_end, w.item + w.n_tiles);
+    const int wt = w.tile_lo + (int)(u - w.item), we = wt + (int)(ue - u);
+    const int pos0 = w.req.len - w.req.n, len = w.req.len;  // position of query 0
+    // Queries: this lane's fragments (row g of each eight) in fp16, bf16 ones divided by the power
+    // of two of the row's largest, which is exact but for numbers 2^-14 below it.
     uint32_t qf[NT][NW][4];
-    float qs[NT][NG][2];
+    float qs[NT][NG][2], qo[NT][NG][2];  // this lane's columns: sums of the queries, and minus the
+                                         // sums weighted with the codes' offsets
+    float cf[NT][2];                     // score scale, in units of log2
     int col_pos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = rb * ROWS + nt * 8 + g;
-      const int j = row / p.G, h = row - j * p.G;
-      const bool live = j < req.n;
-      const uint16_t* qrow = p.q + (p.query_start ? (int64_t)(req.start + j) * p.q_t : r * p.q_r + j * p.q_t) +
-                             (int64_t)(kvh * p.G + h) * p.q_h;
-      float sum[NG] = {};
+      const int row = w.rb * ROWS + nt * 8 + g;
+      const int j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
+      const uint16_t* qrow = p.q + (p.query_start ? (int64_t)(w.req.start + j) * p.q_t : w.r * p.q_r + j * p.q_t) +
+                             (int64_t)(w.kvh * p.G + h) * p.q_h;
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) v = *reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + c));
+        if (j < w.req.n) v = *reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + c));
         qf[nt][i][0] = v.x, qf[nt][i][1] = v.y, qf[nt][i][2] = v.z, qf[nt][i][3] = v.w;
+      }
+      float unit = 1.0f;
+      if (Kv4Nib<T>::kFullRange) {
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a, b;
+            unpack2<T>(qf[nt][i][e], a, b);
+            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+          }
+        big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
+        // the power of two at or below `big`, within 2^+-120; an infinite or NaN row stays what it is
+        const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -120), 120);
+        unit = __uint_as_float((uint32_t)(127 + ex) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a, b;
+            unpack2<T>(qf[nt][i][e], a, b);
+            qf[nt][i][e] = Elem<__half>::from_f2(a * inv, b * inv);
+          }
+      }
+      float sum[NG] = {}, off[NG] = {};
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float a, b;
-          unpack2<T>(qf[nt][i][e], a, b);
+          unpack2<__half>(qf[nt][i][e], a, b);
           sum[i / WPG] += a + b;
+          off[i / WPG] -= (e & 1 ? 64.0f : 1024.0f) * (a + b);
         }
-      }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         sum[k] += __shfl_xor_sync(~0u, sum[k], 1);
         sum[k] += __shfl_xor_sync(~0u, sum[k], 2);
-        qs[nt][k][0] = __shfl_sync(~0u, sum[k], 8 * c);
-        qs[nt][k][1] = __shfl_sync(~0u, sum[k], 8 * c + 4);
+        off[k] += __shfl_xor_sync(~0u, off[k], 1);
+        off[k] += __shfl_xor_sync(~0u, off[k], 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          qs[nt][k][e] = __shfl_sync(~0u, sum[k], 8 * c + 4 * e);
+          qo[nt][k][e] = __shfl_sync(~0u, off[k], 8 * c + 4 * e);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) col_pos[nt][e] = pos0 + (rb * ROWS + nt * 8 + 2 * c + e) / p.G;
+      for (int e = 0; e < 2; ++e) {
+        cf[nt][e] = p.scale_log2 * __shfl_sync(~0u, unit, 8 * c + 4 * e);
+        col_pos[nt][e] = pos0 + (int)((uint32_t)(w.rb * ROWS + nt * 8 + 2 * c + e) / (uint32_t)p.G);
+      }
     }
     // Tiles in [full_lo, full_hi) are visible to every row of the block.
-    const int last_j = min((rb * ROWS + ROWS - 1) / p.G, req.n - 1);
-    const int full_hi = (max(0, pos0 + rb * ROWS / p.G + 1)) / kTile;
+    const int last_j = min((int)((uint32_t)(w.rb * ROWS + ROWS - 1) / (uint32_t)p.G), w.req.n - 1);
+    const int full_hi = max(0, pos0 + (int)((uint32_t)(w.rb * ROWS) / (uint32_t)p.G) + 1) / kTile;
     const int full_lo = p.window > 0 ? (max(0, pos0 + last_j - p.window + 1) + kTile - 1) / kTile : 0;
 
     float out[NW][2][NT][4];
@@ -377,7 +338,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4At
       }
     }
 
-    int stage = 0;
     for (int tile = wt; tile < we; ++tile) {
       mbar_wait(&s_bar[warp][stage], (parity >> stage) & 1u);
       parity ^= 1u << stage;
@@ -398,17 +358,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4At
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][e] = -Nib<T>::kOffset * qs[nt][grp][e & 1];
+            for (int e = 0; e < 4; ++e) acc[nt][e] = qo[nt][grp][e & 1];
 #pragma unroll
           for (int i = grp * WPG; i < (grp + 1) * WPG; ++i) {
-            const uint32_t a0[4] = {Nib<T>::template pair<0>(wa[i]), Nib<T>::template pair<0>(wb[i]),
-                                    Nib<T>::template pair<1>(wa[i]), Nib<T>::template pair<1>(wb[i])};
-            const uint32_t a1[4] = {Nib<T>::template pair<2>(wa[i]), Nib<T>::template pair<2>(wb[i]),
-                                    Nib<T>::template pair<3>(wa[i]), Nib<T>::template pair<3>(wb[i])};
+            uint32_t a0[4], a1[4];
+            code_pairs(wa[i], a0[0], a0[2], a1[0], a1[2]);
+            code_pairs(wb[i], a0[1], a0[3], a1[1], a1[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816<T>(acc[nt], a0, qf[nt][i][0], qf[nt][i][1]);
-              mma16816<T>(acc[nt], a1, qf[nt][i][2], qf[nt][i][3]);
+              mma16816(acc[nt], a0, qf[nt][i][0], qf[nt][i][1]);
+              mma16816(acc[nt], a1, qf[nt][i][2], qf[nt][i][3]);
             }
           }
           float sa, ma, sb, mb;
@@ -418,14 +377,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4At
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = fmaf(e < 2 ? sa : sb, acc[nt][e], (e < 2 ? ma : mb) * qs[nt][grp][e & 1]);
-              s[m][nt][e] = grp ? s[m][nt][e] + v : v;
+              const float v = (e < 2 ? ma : mb) * qs[nt][grp][e & 1];
+              s[m][nt][e] = fmaf(e < 2 ? sa : sb, acc[nt][e], grp ? s[m][nt][e] + v : v);
             }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][nt][e] *= p.scale_log2;
+          for (int e = 0; e < 4; ++e) s[m][nt][e] *= cf[nt][e & 1];
       }
       const bool whole = tile >= full_lo && tile < full_hi;
       if (!whole) {
@@ -436,51 +395,76 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4At
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int t = tile * kTile + m * kKv4Rec + g + (e < 2 ? 0 : 8), pos = col_pos[nt][e & 1];
-              const bool seen = t <= pos && t < req.len && (p.window <= 0 || t > pos - p.window);
+              const bool seen = t <= pos && t < len && (p.window <= 0 || t > pos - p.window);
               if (!seen) s[m][nt][e] = -INFINITY;
             }
       }
-      // ---- running maximum and rescale
-      float scale_old[NT][2], ref[NT][2];
+      // ---- the values' parameters.  The reference exponent is that of p s, so that the weights
+      // p s are at most 1 and fp16 holds them whatever the scales.
+      float sv[2][2][NG], mv[2][2][NG], lg[2][2];  // record, key g or g + 8
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint32_t pv[NG];
+          lds_words<NG>(rec + m * REC + 16 * D + 64 * NG + (g + 8 * y) * NG * 4, pv);
+          float widest = 0.0f;
+#pragma unroll
+          for (int grp = 0; grp < NG; ++grp) {
+            unpack2<T>(pv[grp], sv[m][y][grp], mv[m][y][grp]);
+            // A scale of zero goes with codes of zero; any scale then stands for the same numbers.
+            if (sv[m][y][grp] == 0.0f) sv[m][y][grp] = fmaxf(fabsf(mv[m][y][grp]), 1e-20f);
+            widest = fmaxf(widest, sv[m][y][grp]);
+          }
+          lg[m][y] = log2_approx(widest);
+        }
+      if (!whole) {  // a key that no row sees may carry anything
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if (!(fabsf(lg[m][y]) < 1e9f)) lg[m][y] = 0.0f;
+      }
+      // ---- running reference and rescale
       bool grew = false;
+      float now[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+          float m = fmaxf(fmaxf(s[0][nt][e] + lg[0][0], s[0][nt][e + 2] + lg[0][1]),
+                          fmaxf(s[1][nt][e] + lg[1][0], s[1][nt][e + 2] + lg[1][1]));
           m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
           m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
           m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-          m = fmaxf(m, top[nt][e]);
+          now[nt][e] = fmaxf(m, top[nt][e]);
           grew |= m > top[nt][e];
-          ref[nt][e] = m == -INFINITY ? 0.0f : m;
-          scale_old[nt][e] = exp2f(top[nt][e] - ref[nt][e]);
-          top[nt][e] = m;
         }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            sum[nt][e] *= scale_old[nt][e];
+            const float f = kv4_exp2(top[nt][e] - (now[nt][e] == -INFINITY ? 0.0f : now[nt][e]));
+            top[nt][e] = now[nt][e];
+            sum[nt][e] *= f;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) bias[nt][k][e] *= scale_old[nt][e];
+            for (int k = 0; k < NG; ++k) bias[nt][k][e] *= f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i)
+#pragma unroll
+              for (int m = 0; m < 2; ++m) out[i][m][nt][e] *= f, out[i][m][nt][e + 2] *= f;
           }
-#pragma unroll
-          for (int i = 0; i < NW; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) out[i][m][nt][e] *= scale_old[nt][e & 1];
-        }
       }
+      float ref[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];
       // ---- probabilities, and the products with the values
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const uint8_t* k = rec + m * REC;
-        uint32_t pa[NG], pb[NG];
-        lds_words<NG>(k + 16 * D + 64 * NG + g * NG * 4, pa);
-        lds_words<NG>(k + 16 * D + 64 * NG + (g + 8) * NG * 4, pb);
         uint32_t va[NW], vb[NW];  // tokens 0..7 and 8..15 of the record
         if constexpr (D == 128) {
           lds_words<4>(k + 8 * D + lane * 16, va);
@@ -490,214 +474,244 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn_split_kernel(const Kv4At
           lds_words<4>(k + 8 * D + lane * 16, v4);
           va[0] = v4[0], va[1] = v4[1], vb[0] = v4[2], vb[1] = v4[3];
         }
-        uint32_t pf[NT][NG][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float pr[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            pr[e] = exp2f(s[m][nt][e] - ref[nt][e & 1]);
-            sum[nt][e & 1] += pr[e];
+            s[m][nt][e] = kv4_exp2(s[m][nt][e] - ref[nt][e & 1]);
+            sum[nt][e & 1] += s[m][nt][e];
+          }
+        uint32_t pf[NT][NG][2];
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          // The offset part p (m + 8 s) is formed from the rounded weight x = p s as x (m / s + 8),
+          // so that both parts of p v carry the same rounding and a value near zero keeps a small
+          // error; where the offset is far larger than the scale, from p itself, so that a weight
+          // too small for fp16 loses nothing of it.
+          float r[2], z[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float q = quotient(mv[m][y][grp], sv[m][y][grp]) + 8.0f;
+            const bool small = fabsf(q) <= 16.0f;
+            r[y] = small ? q : 0.0f;
+            z[y] = small ? 0.0f : fmaf(8.0f, sv[m][y][grp], mv[m][y][grp]);
           }
 #pragma unroll
-          for (int grp = 0; grp < NG; ++grp) {
-            float sa, ma, sb, mb;
-            unpack2<T>(pa[grp], sa, ma);
-            unpack2<T>(pb[grp], sb, mb);
-            // (m + 8 s) / s: the offset part is formed from the rounded weight, so that both
-            // parts of p v carry the same rounding and a value near zero keeps a small error.
-            // A weight below the type's normal range (or a scale of zero) says nothing about p.
-            const float ra = quotient(ma, sa) + 8.0f, rb = quotient(mb, sb) + 8.0f;
-            const float ca = fmaf(8.0f, sa, ma), cb = fmaf(8.0f, sb, mb);
-            float w[4], b[4];
+          for (int nt = 0; nt < NT; ++nt) {
+            float x[4], b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[e] = pr[e] * (e < 2 ? sa : sb);
-              // A key that is not seen may carry a NaN or an infinity as its parameters.
-              if (!whole && s[m][nt][e] == -INFINITY) w[e] = 0.0f;
-            }
-            const uint32_t w01 = Elem<T>::from_f2(w[0], w[1]), w23 = Elem<T>::from_f2(w[2], w[3]);
-            unpack2<T>(w01, b[0], b[1]);
-            unpack2<T>(w23, b[2], b[3]);
+            for (int e = 0; e < 4; ++e) x[e] = s[m][nt][e] * sv[m][e >> 1][grp];
+            if (!whole) {  // a key that is not seen may carry NaN parameters
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              b[e] = w[e] < Nib<T>::kMinNormal ? pr[e] * (e < 2 ? ca : cb) : b[e] * (e < 2 ? ra : rb);
-              if (!whole && s[m][nt][e] == -INFINITY) b[e] = 0.0f;
+              for (int e = 0; e < 4; ++e)
+                if (s[m][nt][e] == 0.0f) x[e] = 0.0f;
             }
-            bias[nt][grp][0] += b[0] + b[2];
-            bias[nt][grp][1] += b[1] + b[3];
+            const uint32_t w01 = Elem<__half>::from_f2(x[0], x[1]), w23 = Elem<__half>::from_f2(x[2], x[3]);
+            unpack2<__half>(w01, b[0], b[1]);
+            unpack2<__half>(w23, b[2], b[3]);
+            if (whole) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                bias[nt][grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][nt][e], z[e >> 1], bias[nt][grp][e & 1]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (s[m][nt][e] != 0.0f)
+                  bias[nt][grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][nt][e], z[e >> 1], bias[nt][grp][e & 1]));
+            }
             pf[nt][grp][0] = movmatrix_trans(w01);
             pf[nt][grp][1] = movmatrix_trans(w23);
           }
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          const uint32_t a0[4] = {Nib<T>::centred(Nib<T>::template pair<0>(va[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<1>(va[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<0>(vb[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<1>(vb[i]))};
-          const uint32_t a1[4] = {Nib<T>::centred(Nib<T>::template pair<2>(va[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<3>(va[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<2>(vb[i])),
-                                  Nib<T>::centred(Nib<T>::template pair<3>(vb[i]))};
+          uint32_t a0[4], a1[4];
+          code_pairs(va[i], a0[0], a0[1], a1[0], a1[1]);
+          code_pairs(vb[i], a0[2], a0[3], a1[2], a1[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a0[e] = sub_f16x2(a0[e], e & 1 ? kCentreHigh : kCentreLow);
+            a1[e] = sub_f16x2(a1[e], e & 1 ? kCentreHigh : kCentreLow);
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816<T>(out[i][0][nt], a0, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
-            mma16816<T>(out[i][1][nt], a1, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
+            mma16816(out[i][0][nt], a0, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
+            mma16816(out[i][1][nt], a1, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
           }
         }
       }
       __syncwarp();  // every lane has read this stage
-      if (tile + kStages < we) issue(tile + kStages, stage);
+      copy_next();
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
-    // ---- join the warps: maxima and sums through shared memory, outputs by a tree
+    // ---- the piece's sums over the keys
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           sum[nt][e] += __shfl_xor_sync(~0u, sum[nt][e], o);
 #pragma unroll
           for (int k = 0; k < NG; ++k) bias[nt][k][e] += __shfl_xor_sync(~0u, bias[nt][k][e], o);
         }
-        if (g == 0) {
-          s_max[warp][nt * 8 + 2 * c + e] = top[nt][e];
-          s_sum[warp][nt * 8 + 2 * c + e] = sum[nt][e];
-        }
-      }
-    __syncthreads();
-    float all_top[NT][2], all_sum[NT][2];
+    const bool complete = u == w.item && ue == w.item + w.n_tiles;
+    const int slot = ue == run_end;
+    float* part = part_at(warp, slot);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int col = nt * 8 + 2 * c + e;
-        float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_max[w][col]);
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) l += s_sum[w][col] * exp2f(s_max[w][col] - ref);
-        all_top[nt][e] = m;
-        all_sum[nt][e] = l;
-        const float f = exp2f(top[nt][e] - ref);
-#pragma unroll
-        for (int i = 0; i < NW; ++i)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            out[i][x][nt][e] = (out[i][x][nt][e] + bias[nt][i / WPG][e]) * f;
-            out[i][x][nt][e + 2] = (out[i][x][nt][e + 2] + bias[nt][i / WPG][e]) * f;
-          }
-      }
-    constexpr int PER = NW * 2 * NT * 4;  // outputs per lane
-    float* flat = &out[0][0][0][0];
-#pragma unroll
-    for (int half = kWarps / 2; half >= 1; half >>= 1) {
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) s_out[((warp - half) * PER + k) * 32 + lane] = flat[k];
-      }
-      __syncthreads();
-      if (warp < half) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) flat[k] += s_out[(warp * PER + k) * 32 + lane];
-      }
-      __syncthreads();
-    }
-
-    // ---- write the item, or this CTA's part of it
-    const auto store = [&](int row, int dim, const float (&v)[4], float l) {
-      const int j = row / p.G, h = row - j * p.G;
-      if (j >= req.n) return;
-      const float inv = l > 0.0f ? 1.0f / l : l;  // nothing seen: zeros; NaN stays
-      uint2 o;
-      o.x = Elem<T>::from_f2(v[0] * inv, v[1] * inv);
-      o.y = Elem<T>::from_f2(v[2] * inv, v[3] * inv);
-      *reinterpret_cast<uint2*>(p.out + (int64_t)(req.start + j) * p.o_t + (int64_t)(kvh * p.G + h) * D + dim) = o;
-    };
-    const bool complete = u == item && ue == item + n_tiles;
-    if (complete) {
-      if (warp == 0) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
+        if (complete) {
+          const int row = w.rb * ROWS + col, j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
+          const float inv = sum[nt][e] > 0.0f ? 1.0f / sum[nt][e] : sum[nt][e];  // nothing seen: zeros; NaN stays
+          uint16_t* o = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + h) * D + 4 * g;
+          if (j < w.req.n) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-              const float v[4] = {out[i][0][nt][e], out[i][0][nt][e + 2], out[i][1][nt][e], out[i][1][nt][e + 2]};
-              store(rb * ROWS + nt * 8 + 2 * c + e, 32 * i + 4 * g, v, all_sum[nt][e]);
+              const float b = bias[nt][i / WPG][e];
+              uint2 v;
+              v.x = Elem<T>::from_f2((out[i][0][nt][e] + b) * inv, (out[i][0][nt][e + 2] + b) * inv);
+              v.y = Elem<T>::from_f2((out[i][1][nt][e] + b) * inv, (out[i][1][nt][e + 2] + b) * inv);
+              *reinterpret_cast<uint2*>(o + 32 * i) = v;
             }
-      }
-    } else {
-      constexpr int SLOT = ROWS * (D + 2);
-      const long long first = ((item + 1) * ctas - 1) / total;
-      const long long last = ((item + n_tiles) * ctas - 1) / total;
-      float* part = p.partial + (2 * cta + (item < u0 ? 0 : 1)) * SLOT;
-      if (warp == 0) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = nt * 8 + 2 * c + e;
-            if (g == 0) {
-              part[col] = all_top[nt][e];
-              part[ROWS + col] = all_sum[nt][e];
-            }
-#pragma unroll
-            for (int i = 0; i < NW; ++i)
-              *reinterpret_cast<float4*>(part + 2 * ROWS + col * D + 32 * i + 4 * g) =
-                  make_float4(out[i][0][nt][e], out[i][0][nt][e + 2], out[i][1][nt][e], out[i][1][nt][e + 2]);
           }
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) s_last = atomicAdd(p.counters + first, 1) == (int)(last - first);
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        // Four dims of one column per thread; the parts in the order of the CTAs.
-        for (int k = tid; k < ROWS * D / 4; k += kThreads) {
-          const int col = k / (D / 4), dim = (k % (D / 4)) * 4;
-          float m = -INFINITY, l = 0.0f;
-          for (long long x = first; x <= last; ++x)
-            m = fmaxf(m, __ldcg(p.partial + (2 * x + (x == first ? 1 : 0)) * SLOT + col));
-          const float ref = m == -INFINITY ? 0.0f : m;
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-          for (long long x = first; x <= last; ++x) {
-            const float* q = p.partial + (2 * x + (x == first ? 1 : 0)) * SLOT;
-            const float f = exp2f(__ldcg(q + col) - ref);
-            l += __ldcg(q + ROWS + col) * f;
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(q + 2 * ROWS + col * D + dim));
-            v[0] += o.x * f, v[1] += o.y * f, v[2] += o.z * f, v[3] += o.w * f;
+        } else {
+          if (g == 0) {
+            s_max[warp][slot][col] = top[nt][e];
+            s_sum[warp][slot][col] = sum[nt][e];
           }
-          store(rb * ROWS + col, dim, v, l);
+#pragma unroll
+          for (int i = 0; i < NW; ++i) {
+            const float b = bias[nt][i / WPG][e];
+            *reinterpret_cast<float4*>(part + col * (D + 4) + 32 * i + 4 * g) = make_float4(
+                out[i][0][nt][e] + b, out[i][0][nt][e + 2] + b, out[i][1][nt][e] + b, out[i][1][nt][e + 2] + b);
+          }
         }
-        if (tid == 0) p.counters[first] = 0;
       }
-      __syncthreads();  // s_last is written again by the next piece
-    }
-
-    // ---- next item
+    if (!complete && lane == 0)
+      s_info[warp][slot] = PartInfo{w.item, w.n_tiles, w.rb * ROWS, w.req.start, w.req.n, w.kvh * p.G};
     u = ue;
-    if (u >= u1) break;
-    item += n_tiles;
-    if (++rb == blocks) {
-      rb = 0;
-      if (++kvh == p.c.n_kv) {
-        kvh = 0;
-        blocks = 0;
-        while (blocks == 0 && ++r < p.R) {
-          req = load_request(p, r);
-          blocks = (req.n * p.G + ROWS - 1) / ROWS;
+    if (u < run_end) {
+      Work x = w;
+      __syncwarp();
+      const bool more = x.next(p);
+      if (lane == 0) s_item[warp] = x;
+      __syncwarp();
+      if (!more) break;
+    }
+  }
+
+  // ---- join the warps' parts, item by item: four dims of one column per thread
+  __syncthreads();
+  const Work& any = s_item[0];
+  constexpr int SLOT = ROWS * (D + 2);
+  const auto store = [&](const PartInfo& x, int col, int dim, float4 v, float l) {
+    const int row = x.row0 + col, j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
+    if (j >= x.n) return;
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    uint2 o;
+    o.x = Elem<T>::from_f2(v.x * inv, v.y * inv);
+    o.y = Elem<T>::from_f2(v.z * inv, v.w * inv);
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(x.start + j) * p.o_t + (int64_t)(x.head0 + h) * D + dim) = o;
+  };
+  int shared_at[2] = {-1, -1};  // entries (warp * 2 + slot) of the items shared with other CTAs
+  for (int x = 0; x < 2 * WARPS;) {
+    const PartInfo& info = s_info[x >> 1][x & 1];
+    if (info.item < 0) {
+      ++x;
+      continue;
+    }
+    int y = x + 1, end = y;  // entries [x, end) belong to the item
+    for (; y < 2 * WARPS; ++y) {
+      const long long it = s_info[y >> 1][y & 1].item;
+      if (it >= 0 && it != info.item) break;
+      if (it >= 0) end = y + 1;
+    }
+    const bool here = info.item >= any.u0 && info.item + info.n_tiles <= any.u1;
+    const int side = info.item < any.u0 ? 0 : 1;
+    if (!here) shared_at[side] = x;
+    float* part = p.partial + (int64_t)(2 * (int)blockIdx.x + side) * SLOT;
+    for (int k = tid; k < ROWS * D / 4; k += THREADS) {
+      const int col = k / (D / 4), dim = k % (D / 4) * 4;
+      float m = -INFINITY, l = 0.0f;
+      for (int z = x; z < end; ++z)
+        if (s_info[z >> 1][z & 1].item >= 0) m = fmaxf(m, s_max[z >> 1][z & 1][col]);
+      const float to = m == -INFINITY ? 0.0f : m;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int z = x; z < end; ++z) {
+        if (s_info[z >> 1][z & 1].item < 0) continue;
+        const float f = kv4_exp2(s_max[z >> 1][z & 1][col] - to);
+        const float4 o = *reinterpret_cast<const float4*>(part_at(z >> 1, z & 1) + col * (D + 4) + dim);
+        l = fmaf(s_sum[z >> 1][z & 1][col], f, l);
+        v.x = fmaf(o.x, f, v.x), v.y = fmaf(o.y, f, v.y), v.z = fmaf(o.z, f, v.z), v.w = fmaf(o.w, f, v.w);
+      }
+      if (here) {
+        store(info, col, dim, v, l);
+      } else {
+        if (dim == 0) {
+          part[col] = m;
+          part[ROWS + col] = l;
         }
-        if (blocks == 0) break;  // lengths that changed under the kernel
+        *reinterpret_cast<float4*>(part + 2 * ROWS + col * D + dim) = v;
       }
     }
-    block_tiles<ROWS>(p, req, rb, tile_lo, n_tiles);
+    x = y;
+  }
+  if (shared_at[0] < 0 && shared_at[1] < 0) return;
+
+  // ---- items shared with other CTAs: the last to arrive adds the parts, in the order of the CTAs
+  __threadfence();
+  __syncthreads();
+  if (tid < 2 && shared_at[tid] >= 0) {
+    const PartInfo& info = s_info[shared_at[tid] >> 1][shared_at[tid] & 1];
+    const int fc = any.owner(info.item), lc = any.owner(info.item + info.n_tiles - 1);
+    const bool last = atomicAdd(p.counters + fc, 1) == lc - fc;
+    if (last) p.counters[fc] = 0;
+    s_last[tid] = last;
+  }
+  __syncthreads();
+  for (int side = 0; side < 2; ++side) {
+    if (shared_at[side] < 0 || !s_last[side]) continue;
+    __threadfence();
+    const PartInfo& info = s_info[shared_at[side] >> 1][shared_at[side] & 1];
+    const int fc = any.owner(info.item), lc = any.owner(info.item + info.n_tiles - 1);
+    const auto slot = [&](int x) { return p.partial + (int64_t)(2 * x + (x == fc ? 1 : 0)) * SLOT; };
+    for (int k = tid; k < ROWS * D / 4; k += THREADS) {
+      const int col = k / (D / 4), dim = k % (D / 4) * 4;
+      float m = -INFINITY, l = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      // Eight parts at a time: their loads are in flight together.
+      for (int x0 = fc; x0 <= lc; x0 += 8) {
+        float pm[8], pl[8];
+        float4 po[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float* q = slot(min(x0 + y, lc));
+          pm[y] = x0 + y <= lc ? __ldcg(q + col) : -INFINITY;
+          pl[y] = __ldcg(q + ROWS + col);
+          po[y] = __ldcg(reinterpret_cast<const float4*>(q + 2 * ROWS + col * D + dim));
+        }
+        float to = m;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) to = fmaxf(to, pm[y]);
+        const float at = to == -INFINITY ? 0.0f : to;
+        const float old = kv4_exp2(m - at);
+        l *= old, v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+        m = to;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float f = kv4_exp2(pm[y] - at);
+          if (x0 + y > lc) continue;
+          l = fmaf(pl[y], f, l);
+          v.x = fmaf(po[y].x, f, v.x), v.y = fmaf(po[y].y, f, v.y);
+          v.z = fmaf(po[y].z, f, v.z), v.w = fmaf(po[y].w, f, v.w);
+        }
+      }
+      store(info, col, dim, v, l);
+    }
   }
 }
 
@@ -707,8 +721,8 @@ cudaError_t launch_one(const Kv4AttnParams& p, int sms, bool pdl, cudaStream_t s
   const auto kernel = kv4_attn_split_kernel<T, D, NG, NT>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  const int grid = sms * 2 < kKv4MaxGrid ? sms * 2 : kKv4MaxGrid;
-  return kv4_launch(kernel, dim3((unsigned)grid), kThreads, smem, pdl, stream, p);
+  const int grid = sms * (NT == 1 ? 2 : 1) < kKv4MaxGrid ? sms * (NT == 1 ? 2 : 1) : kKv4MaxGrid;
+  return kv4_launch(kernel, dim3((unsigned)grid), warps<D, NG, NT>() * 32, smem, pdl, stream, p);
 }
 
 template <typename T, int NT>

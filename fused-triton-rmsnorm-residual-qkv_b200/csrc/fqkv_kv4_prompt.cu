@@ -30,7 +30,7 @@ constexpr int kPRows = 256;
 constexpr int kPTile = 128;  // keys per step
 constexpr int kPMinTiles = 4;
 
-using Work = Kv4Work<kPRows, kPTile, kPThreads>;
+using Work = Kv4Work<kPRows, kPTile, kPThreads, 1>;
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,

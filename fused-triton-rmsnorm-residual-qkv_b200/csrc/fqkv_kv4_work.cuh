@@ -36,28 +36,40 @@ __device__ __forceinline__ Kv4Request kv4_load_request(const Kv4AttnParams& p, i
   return q;
 }
 
-template <int ROWS, int TILE, int THREADS>
+// x * y / z for the cutting points: 32-bit arithmetic where the product allows it (a 64-bit
+// division costs about 0.3 us of a CTA's start).
+__device__ __forceinline__ long long kv4_muldiv(long long x, long long y, long long z, bool small) {
+  return small ? (long long)((uint32_t)x * (uint32_t)y / (uint32_t)z) : x * y / z;
+}
+
+// POINTS: 1, or the block's warps; the run of the CTA or of each of its warps starts there.
+template <int ROWS, int TILE, int THREADS, int POINTS>
 struct Kv4Work {
   struct Shared {
     long long scan[THREADS / 32];
-    long long found;
-    int r;
+    long long found[POINTS], per_head[POINTS];
+    Kv4Request req[POINTS];
+    int r[POINTS];
   };
 
-  long long total, ctas, u0, u1;  // all tiles, CTAs that have work, this CTA's run
+  long long total, u0, u1;  // all tiles, this CTA's run
+  long long a, b;           // this warp's part of it (POINTS > 1)
   // The current item: request r, KV head, row block; its tiles [tile_lo, tile_lo + n_tiles), the
   // first of which is tile `item` of the batch; row blocks of the request.
-  Kv4Request req;
   long long item;
+  Kv4Request req;
+  int ctas;   // CTAs that have work
+  bool small;  // total * ctas is below 2^32
   int r, kvh, rb, blocks, tile_lo, n_tiles;
 
   // Tiles that row block rb of a request reads (at least one, so that every item is visited).
   // Rows are (query j, head) with row = j * G + head.
   static __device__ __forceinline__ void block_tiles(const Kv4AttnParams& p, const Kv4Request& q, int rb, int& tile_lo,
                                                      int& n_tiles) {
-    const int j0 = rb * ROWS / p.G, j1 = min((rb * ROWS + ROWS - 1) / p.G, q.n - 1);
+    const int j1 = min((int)((uint32_t)(rb * ROWS + ROWS - 1) / (uint32_t)p.G), q.n - 1);
     const int hi = max(0, min(q.len, q.len - q.n + j1 + 1));
-    const int lo = p.window > 0 ? max(0, q.len - q.n + j0 - p.window + 1) : 0;
+    int lo = 0;
+    if (p.window > 0) lo = max(0, q.len - q.n + (int)((uint32_t)(rb * ROWS) / (uint32_t)p.G) - p.window + 1);
     tile_lo = lo / TILE;
     n_tiles = max(1, (hi + TILE - 1) / TILE - tile_lo);
   }
@@ -66,75 +78,156 @@ struct Kv4Work {
     return (q.n * p.G + ROWS - 1) / ROWS;
   }
 
+  // Tiles of one KV head of the lane's request (0 for q.n == 0).  Requests of more than two row
+  // blocks are summed by the whole warp, one after the other.  Called by whole warps.
   static __device__ __forceinline__ long long head_tiles(const Kv4AttnParams& p, const Kv4Request& q) {
-    const int n = row_blocks(p, q);
+    const int lane = threadIdx.x & 31, n = row_blocks(p, q);
     long long sum = 0;
-    for (int rb = 0; rb < n; ++rb) {
-      int lo, tiles;
-      block_tiles(p, q, rb, lo, tiles);
-      sum += tiles;
+    int lo, tiles;
+    if (n > 0 && n <= 2) {
+      block_tiles(p, q, 0, lo, tiles);
+      sum = tiles;
+      if (n == 2) {
+        block_tiles(p, q, 1, lo, tiles);
+        sum += tiles;
+      }
+    }
+    for (uint32_t big = __ballot_sync(~0u, n > 2); big; big &= big - 1) {
+      const int owner = __ffs(big) - 1;
+      Kv4Request o;
+      o.start = 0;
+      o.n = __shfl_sync(~0u, q.n, owner);
+      o.len = __shfl_sync(~0u, q.len, owner);
+      const int on = row_blocks(p, o);
+      long long part = 0;
+      for (int rb = lane; rb < on; rb += 32) {
+        block_tiles(p, o, rb, lo, tiles);
+        part += tiles;
+      }
+#pragma unroll
+      for (int k = 16; k; k >>= 1) part += __shfl_xor_sync(~0u, part, k);
+      if (lane == owner) sum = part;
     }
     return sum;
+  }
+
+  // First tile of the run of point k.
+  __device__ __forceinline__ long long point(int k) const {
+    return POINTS == 1 ? u0 : u0 + kv4_muldiv(k, u1 - u0, POINTS, small);
   }
 
   // Called by the whole block.  False: this CTA has no work.
   __device__ __forceinline__ bool locate(const Kv4AttnParams& p, Shared& s, int max_ctas, int min_tiles) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    long long mine = 0, sum = 0;
-    for (int k = tid; k < p.R; k += THREADS) {
-      mine = head_tiles(p, kv4_load_request(p, k)) * p.c.n_kv;
-      sum += mine;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) s.scan[warp] = sum;
-    __syncthreads();
+    const Kv4Request none{0, 0, 0};
+    // Pass 0 sums; the pass that finds the run's request is the same one when all requests fit the
+    // block, a second walk over the chunks otherwise.
+    const bool one = p.R <= THREADS;
+    Kv4Request q = none;
+    long long heads = 0, before = 0;
     total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) total += s.scan[w];
-    ctas = max(1ll, min((long long)max_ctas, total / min_tiles));
-    const long long cta = blockIdx.x;
-    if (cta >= ctas || total == 0) return false;
-    u0 = cta * total / ctas;
-    u1 = (cta + 1) * total / ctas;
-    long long base = 0;
     for (int k0 = 0; k0 < p.R; k0 += THREADS) {
       const int k = k0 + tid;
-      const long long n = p.R <= THREADS ? mine : k < p.R ? head_tiles(p, kv4_load_request(p, k)) * p.c.n_kv : 0;
-      long long v = n;
+      q = k < p.R ? kv4_load_request(p, k) : none;
+      heads = head_tiles(p, q);
+      long long v = heads * p.c.n_kv;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(~0u, v, o);
         if (lane >= o) v += u;
       }
-      __syncthreads();
       if (lane == 31) s.scan[warp] = v;
       __syncthreads();
-      long long before = base;
+      before = total + v - heads * p.c.n_kv;
+#pragma unroll
       for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += s.scan[w];
-        base += s.scan[w];
+        total += s.scan[w];
       }
-      if (before + v - n <= u0 && u0 < before + v) {
-        s.r = k;
-        s.found = before + v - n;
+      if (!one) __syncthreads();
+    }
+    ctas = (int)max(1ll, min((long long)max_ctas, total / min_tiles));
+    small = total < (1ll << 32) / 1024;
+    const int cta = blockIdx.x;
+    if (cta >= ctas || total == 0) return false;
+    u0 = kv4_muldiv(cta, total, ctas, small);
+    u1 = kv4_muldiv(cta + 1, total, ctas, small);
+    if (one) {
+      publish(s, q, tid, before, heads, p.c.n_kv);
+    } else {
+      long long base = 0;
+      for (int k0 = 0; k0 < p.R && base < u1; k0 += THREADS) {
+        const int k = k0 + tid;
+        q = k < p.R ? kv4_load_request(p, k) : none;
+        heads = head_tiles(p, q);
+        long long v = heads * p.c.n_kv;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long u = __shfl_up_sync(~0u, v, o);
+          if (lane >= o) v += u;
+        }
+        __syncthreads();
+        if (lane == 31) s.scan[warp] = v;
+        __syncthreads();
+        before = base + v - heads * p.c.n_kv;
+        for (int w = 0; w < THREADS / 32; ++w) {
+          if (w < warp) before += s.scan[w];
+          base += s.scan[w];
+        }
+        publish(s, q, k, before, heads, p.c.n_kv);
       }
-      if (base > u0) break;
     }
     __syncthreads();
-    r = s.r;
-    item = s.found;
-    req = kv4_load_request(p, r);
+    const int at_point = POINTS == 1 ? 0 : warp;
+    a = point(at_point);
+    b = POINTS == 1 ? u1 : point(at_point + 1);
+    r = s.r[at_point];
+    req = s.req[at_point];
+    item = s.found[at_point];
     blocks = row_blocks(p, req);
-    const long long per_head = head_tiles(p, req);
-    kvh = (int)((u0 - item) / per_head);
-    item += kvh * per_head;
-    for (rb = 0;; ++rb) {
-      block_tiles(p, req, rb, tile_lo, n_tiles);
-      if (u0 < item + n_tiles) break;
-      item += n_tiles;
+    const long long per_head = s.per_head[at_point];
+    kvh = 0;
+    while (a - item >= per_head) {  // fewer steps than KV heads, and no division
+      item += per_head;
+      ++kvh;
     }
+    // The row block: each lane sums its own share of 32 blocks at a time.
+    for (rb = 0;; rb += 32) {
+      int lo, tiles = 0;
+      if (rb + lane < blocks) block_tiles(p, req, rb + lane, lo, tiles);
+      int v = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, v, o);
+        if (lane >= o) v += u;
+      }
+      const uint32_t past = __ballot_sync(~0u, a < item + v);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        item += __shfl_sync(~0u, v - tiles, at);
+        rb += at;
+        break;
+      }
+      item += __shfl_sync(~0u, v, 31);
+    }
+    block_tiles(p, req, rb, tile_lo, n_tiles);
     return true;
+  }
+
+  __device__ __forceinline__ void publish(Shared& s, const Kv4Request& q, int k, long long before, long long heads,
+                                          int n_kv) const {
+    const long long after = before + heads * n_kv;
+    if (after <= u0 || before >= u1) return;
+#pragma unroll
+    for (int x = 0; x < POINTS; ++x) {
+      const long long u = point(x);
+      if (before <= u && u < after) {
+        s.r[x] = k;
+        s.found[x] = before;
+        s.per_head[x] = heads;
+        s.req[x] = q;
+      }
+    }
   }
 
   // The item after the current one.  False: none (lengths that changed under the kernel).
@@ -149,7 +242,11 @@ struct Kv4Work {
           req = kv4_load_request(p, r);
           blocks = row_blocks(p, req);
         }
-        if (blocks == 0) return false;
+        if (blocks == 0) {
+          r = p.R - 1;
+          req = Kv4Request{0, 0, 0};
+          return false;
+        }
       }
     }
     block_tiles(p, req, rb, tile_lo, n_tiles);
@@ -158,8 +255,12 @@ struct Kv4Work {
 
   // First and last CTA that have a part of the current item; a CTA's part goes to workspace slot
   // 2 * cta (the item began before its run) or 2 * cta + 1.
-  __device__ __forceinline__ int first_cta() const { return (int)(((item + 1) * ctas - 1) / total); }
-  __device__ __forceinline__ int last_cta() const { return (int)(((item + n_tiles) * ctas - 1) / total); }
+  __device__ __forceinline__ int owner(long long tile) const {
+    return small ? (int)(((uint32_t)(tile + 1) * (uint32_t)ctas - 1) / (uint32_t)total)
+                 : (int)(((tile + 1) * ctas - 1) / total);
+  }
+  __device__ __forceinline__ int first_cta() const { return owner(item); }
+  __device__ __forceinline__ int last_cta() const { return owner(item + n_tiles - 1); }
 };
 
 // Address of record `rec` (16 tokens) of a request for one KV head; null past its last key.
@@ -184,7 +285,7 @@ struct Kv4Nib<__nv_bfloat16> {
   static constexpr float kOffset = 128.0f;  // 0x4300: four mantissa bits of weight 1..8
   static constexpr uint32_t kOffset2 = 0x43004300u;
   static constexpr uint32_t kCentre2 = 0x43084308u;  // 136 = offset + 8
-  static constexpr float kMinNormal = 1e-30f;
+  static constexpr bool kFullRange = true;  // of fp32
   template <int j>
   static __device__ __forceinline__ uint32_t pair(uint32_t w) {
     return ((w >> (4 * j)) & 0x000F000Fu) | kOffset2;
@@ -205,7 +306,7 @@ struct Kv4Nib<__half> {
   static constexpr float kOffset = 64.0f;  // 0x5400: mantissa bits 4..7 have weight 1..8
   static constexpr uint32_t kOffset2 = 0x54005400u;
   static constexpr uint32_t kCentre2 = 0x54805480u;  // 72 = offset + 8
-  static constexpr float kMinNormal = 6.2e-5f;
+  static constexpr bool kFullRange = false;
   template <int j>
   static __device__ __forceinline__ uint32_t pair(uint32_t w) {
     const uint32_t x = j == 0 ? w << 4 : w >> (4 * (j > 0 ? j - 1 : 0));
