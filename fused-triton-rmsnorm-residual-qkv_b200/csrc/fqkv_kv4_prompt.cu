@@ -11,21 +11,24 @@
 // Shape.  A CTA takes 256 query rows of one KV head (all heads that share it, so the keys are
 // unpacked once for them) as two tiles of 128 and walks the keys 128 at a time:
 //   warps 0-3, 4-7   softmax of the two tiles, one row per thread, S and O in TMEM; P goes back
-//                    to TMEM over S and is the A operand of the second product
-//   warps 8-11       4-bit codes from global memory to swizzled shared-memory operands
-//   warp 12          issues the products: S0(j+1) follows P0 V(j), S1(j+1) follows P1 V(j), so
-//                    one tile's softmax runs under the other tile's products
+//                    to TMEM over S and is the A operand of the second product.  The first warp
+//                    of each issues its tile's products, P V(j) and then S(j+1), so one tile's
+//                    softmax runs under the other tile's products
+//   warps 8-11       4-bit codes from global memory to swizzled shared-memory operands, and the
+//                    queries of the next item while the current one ends
+// Twelve warps leave a thread 168 registers: a row's 128 scores are read from TMEM once.
 // The values are stored transposed (dims x keys, K-major) because the cache interleaves tokens
 // in pairs: a thread's eight tokens of one dim are one 16-byte store without any permutation.
 //
-// Bound: per 128 keys the four products take 2048 tensor cycles, the softmax 32768 exponentials
-// (2048 cycles of the special function unit) and the unpacking about 500 issue cycles.
+// Bound: per 128 keys the four products take 2048 tensor cycles and the softmax 32768
+// exponentials, 2048 cycles of the special function unit: a quarter of them is a polynomial
+// on the FMA pipe instead (packed pairs), the scaling and the sums are packed pairs too.
 #include "fqkv_kv4_work.cuh"
 
 namespace fqkv {
 namespace {
 
-constexpr int kPThreads = 416;  // 13 warps: 128 registers a thread
+constexpr int kPThreads = 384;
 constexpr int kPRows = 256;
 constexpr int kPTile = 128;  // keys per step
 constexpr int kPMinTiles = 4;
@@ -57,15 +60,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : FQKV_R8(r, 0), FQKV_R8(r, 8), FQKV_R8(r, 16), FQKV_R8(r, 24)
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      FQKV_W8(r, 0), FQKV_W8(r, 8), FQKV_W8(r, 16), FQKV_W8(r, 24)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -73,38 +67,113 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       FQKV_W8(r, 0), FQKV_W8(r, 8)
       : "memory");
 }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Scores of keys outside [lo, hi) of this chunk become -inf.
-__device__ __forceinline__ void hide32(uint32_t (&r)[32], int lo, int hi) {
+// ------------------------------------------------------------------ packed fp32 pairs
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack64(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// 2^x for a pair, x < 127, on the FMA pipe: x = i + f with i the nearest integer,
+// 2^f by a polynomial (largest relative error 7.5e-5 at degree 3, for P rounded to bf16, 2.6e-6 at
+// degree 4 for fp16; fitted by equalising the error's extremes on [-1/2, 1/2]), i added to the
+// exponent.  Below 2^-125 the result is 2^-125, which is zero beside a row's largest entry.
+template <bool BF16>
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+  float a, b;
+  unpack64(x, a, b);
+  x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+  const uint64_t magic = pack2(12582912.0f, 12582912.0f), minus = pack2(-12582912.0f, -12582912.0f);
+  const uint64_t t = add2(x, magic);  // the integer in the low mantissa bits
+  const uint64_t f = fma2(add2(t, minus), pack2(-1.0f, -1.0f), x);
+  uint64_t r;
+  if constexpr (BF16) {
+    r = fma2(f, pack2(0.05517166852951f, 0.05517166852951f), pack2(0.24261112511158f, 0.24261112511158f));
+    r = fma2(r, f, pack2(0.69326096773148f, 0.69326096773148f));
+    r = fma2(r, f, pack2(0.99992805719376f, 0.99992805719376f));
+  } else {
+    r = fma2(f, pack2(0.00957010220736f, 0.00957010220736f), pack2(0.05591785907745f, 0.05591785907745f));
+    r = fma2(r, f, pack2(0.24024744331837f, 0.24024744331837f));
+    r = fma2(r, f, pack2(0.69312179088593f, 0.69312179088593f));
+    r = fma2(r, f, pack2(0.99999928474426f, 0.99999928474426f));
+  }
+  float ta, tb;
+  unpack64(t, ta, tb);
+  unpack64(r, a, b);
+  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
+               __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+}
+
+// Scores of keys outside [lo, hi) of a chunk become -inf.
+__device__ __forceinline__ void hide32(uint32_t* r, int lo, int hi) {
 #pragma unroll
   for (int k = 0; k < 32; ++k)
     if (k < lo || k >= hi) r[k] = 0xFF800000u;
 }
-__device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
-  float m[4];
-#pragma unroll
-  for (int k = 0; k < 32; ++k) m[k & 3] = k < 4 ? __uint_as_float(r[k]) : fmaxf(m[k & 3], __uint_as_float(r[k]));
-  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-}
-// P = exp2(c S - off) of 32 keys to 16 columns at `dst`; returns their fp32 sum.
-template <typename T>
-__device__ __forceinline__ float exp32(const uint32_t (&r)[32], float c, float off, uint32_t dst) {
+// P = exp2(c S - off) of 32 keys to 16 columns at `dst`, added to `sum` in fp32.
+template <typename T, bool BF16>
+__device__ __forceinline__ void exp32(const uint32_t* r, uint64_t c, uint64_t off, uint32_t dst, uint64_t (&sum)[2]) {
   uint32_t pk[16];
-  float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const float x = kv4_exp2(fmaf(__uint_as_float(r[2 * k]), c, -off));
-    const float y = kv4_exp2(fmaf(__uint_as_float(r[2 * k + 1]), c, -off));
-    a[2 * (k & 1)] += x, a[2 * (k & 1) + 1] += y;
-    pk[k] = Elem<T>::from_f2(x, y);
+    uint64_t x = fma2(pack2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), c, off);
+    float a, b;
+    if (k % 4 == 3) {
+      x = exp2_poly2<BF16>(x);
+      unpack64(x, a, b);
+    } else {
+      unpack64(x, a, b);
+      a = kv4_exp2(a);
+      b = kv4_exp2(b);
+      x = pack2(a, b);
+    }
+    sum[k & 1] = add2(sum[k & 1], x);
+    pk[k] = Elem<T>::from_f2(a, b);
   }
   tmem_st16(dst, pk);
-  return (a[0] + a[1]) + (a[2] + a[3]);
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// One arrival for a warp whose lanes have all got here.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 struct Bars {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t k_full[2], v_full[2];    // operands of a step written: one arrival per unpacking warp
+  uint64_t k_empty[2], v_empty[2];  // and read by both tiles' products
+  uint64_t q_full;                  // the queries of an item
+  uint64_t s_full[2], o_done[2];    // a tile's scores; its part of O
 };
 
 // Whether a scale or a minimum (packed pair) is a NaN or an infinity.
@@ -129,33 +198,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
   constexpr int OP = operand_bytes<D>();
   constexpr int REC = kv4_record_bytes(D, NG);
   constexpr int NW = D / 32;
-  constexpr bool kBf16 = sizeof(T) == 2 && Kv4Nib<T>::kOffset == 128.0f;
+  constexpr bool kBf16 = Kv4Nib<T>::kFullRange;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ Work::Shared s_work;
   __shared__ uint32_t s_tmem;
   __shared__ int s_last;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.k_full[i], 128);
-      mbar_init(&bars.v_full[i], 128);
-      mbar_init(&bars.k_empty[i], 1);
-      mbar_init(&bars.v_empty[i], 1);
-      mbar_init(&bars.q_full[i], 128);
+      mbar_init(&bars.k_full[i], 4);
+      mbar_init(&bars.v_full[i], 4);
+      mbar_init(&bars.k_empty[i], 2);
+      mbar_init(&bars.v_empty[i], 2);
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 128);
       mbar_init(&bars.o_done[i], 1);
     }
+    mbar_init(&bars.q_full, 4);
     fence_mbarrier_init_cluster();
   }
   pdl_wait();
   pdl_launch_dependents();
   Work w;
   if (!w.locate(p, s_work, gridDim.x, kPMinTiles)) return;
-  if (warp == 12) {
+  if (warp == 8) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
@@ -163,150 +231,199 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const auto s_col = [&](int t) { return tmem + t * 128; };        // S, and P over it
-  const auto o_col = [&](int t) { return tmem + 256 + t * 128; };  // O
 
   if (warp < 8) {
-    // ================================================================ softmax
+    // ================================================================ softmax and products
     const int t = warp >> 2, row = tid & 127;  // tile, row of the tile = TMEM lane
+    const uint32_t s_tm = tmem + t * 128, o_tm = tmem + 256 + t * 128;  // S (P over it), O
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const bool issuer = (warp & 3) == 0;
     const float c = fabsf(p.scale_log2);
-    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale goes into Q
-    uint32_t s_phase = 0, o_phase = 0;
+    const uint64_t c2 = pack2(c, c);
+    constexpr uint32_t idesc_s = make_idesc_f16(128, 128, kBf16), idesc_o = make_idesc_f16(128, D, kBf16);
+    // Descriptors are one 64-bit base and constant steps (16-byte units).
+    const uint64_t base = make_sw128_desc(smem_u32(smem));
+    uint32_t it = 0, s_phase = 0, o_phase = 0, q_phase = 0;
     bool ok = true;  // after a wait that ran out nothing is waited for, and every barrier is still reached
+    const auto wait = [&](uint64_t* bar, uint32_t phase) { ok = __all_sync(~0u, ok && mbar_wait(bar, phase & 1u)); };
+    // Scores of step x (the issuing warp).
+    const auto issue_s = [&](uint32_t x) {
+      wait(&bars.k_full[x & 1], x >> 1);
+      tc_fence_after();
+      const uint64_t a = base + (uint64_t)(t * (OP >> 4)), b = base + (uint64_t)((2 + (x & 1)) * (OP >> 4));
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = ((k / 4) * 128 * 128 + (k % 4) * 32) >> 4;
+          umma_f16(s_tm, a + off, b + off, idesc_s, k > 0);
+        }
+        umma_commit(&bars.s_full[t]);
+        umma_commit(&bars.k_empty[x & 1]);
+      }
+      __syncwarp();
+    };
+    const auto issue_o = [&](uint32_t x, bool accumulate) {
+      wait(&bars.v_full[x & 1], x >> 1);
+      tc_fence_after();
+      const uint64_t b = base + (uint64_t)((4 + (x & 1)) * (OP >> 4));
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16_ts(o_tm, s_tm + k * 8, b + (((k / 4) * D * 128 + (k % 4) * 32) >> 4), idesc_o, k > 0 || accumulate);
+        umma_commit(&bars.o_done[t]);
+        umma_commit(&bars.v_empty[x & 1]);
+      }
+      __syncwarp();
+    };
+    // First scores of the item (the issuing warp); a tile without rows only lets its steps pass.
+    const auto begin = [&](bool used) {
+      wait(&bars.q_full, q_phase);
+      if (used) issue_s(it);
+    };
+    if (issuer) begin(w.req.n * p.G - w.rb * kPRows > t * 128);
     for (long long u = w.u0; u < w.u1;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
       const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
       const int rows = w.req.n * p.G - w.rb * kPRows;  // live rows of the block
       const int grow = w.rb * kPRows + t * 128 + row;  // row of the request
-      const int j = grow / p.G, h = grow - j * p.G;
+      const int j = (int)((uint32_t)grow / (uint32_t)p.G);
       const bool live = j < w.req.n;
-      const int pos = w.req.len - w.req.n + j;
       const bool tile_used = rows > t * 128;
+      uint16_t* out = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + grow - j * p.G) * D;
       float ref = -INFINITY, sum = 0.0f;
+      q_phase ^= 1u;
       if (tile_used) {
-        // ---- this row of Q into the tile's operand
-        uint8_t* q_tile = smem + t * OP;
-        const uint16_t* q = p.q + (p.query_start ? (int64_t)(w.req.start + j) * p.q_t : w.r * p.q_r + j * p.q_t) +
-                            (int64_t)(w.kvh * p.G + h) * p.q_h;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live) v = *reinterpret_cast<const uint4*>(q + k * 8);
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-          *reinterpret_cast<uint4*>(q_tile + (k / 8) * 128 * 128 + sw128_offset(row, k % 8)) = v;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.q_full[t]);
-
+        const int pos = w.req.len - w.req.n + j;
         const int see_hi = live ? min(pos + 1, w.req.len) : w.req.len;      // keys [see_lo, see_hi)
         const int see_lo = live && p.window > 0 ? max(0, pos - p.window + 1) : 0;
         const bool warp_live = rows > t * 128 + (warp & 3) * 32;
-        for (int tile = first; tile < last; ++tile) {
-          ok = __all_sync(~0u, ok && mbar_wait(&bars.s_full[t], s_phase & 1u));
+        uint64_t sum2[2] = {0, 0};
+        for (int tile = first; tile < last; ++tile, ++it) {
+          wait(&bars.s_full[t], s_phase);
           s_phase ^= 1u;
           tc_fence_after();
           if (warp_live) {
-            // The row's 128 scores are read twice, for the maximum and for the exponentials, 64 at a
-            // time: a thread stays within the 128 registers that 13 warps leave it.
-            uint32_t r0[32], r1[32];
+            uint32_t s[128];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tmem_ld32(s_tm + lane_base + 32 * k, s + 32 * k);
+            tmem_wait_ld();
             const int lo = see_lo - tile * kPTile, hi = see_hi - tile * kPTile;
-            const bool edge = __any_sync(~0u, lo > 0 || hi < kPTile);
-            tmem_ld32(s_col(t) + lane_base, r0);
-            tmem_ld32(s_col(t) + lane_base + 32, r1);
-            tmem_wait_ld();
-            if (edge) hide32(r0, lo, hi), hide32(r1, lo - 32, hi - 32);
-            float top = fmaxf(max32(r0), max32(r1));
-            tmem_ld32(s_col(t) + lane_base + 64, r0);
-            tmem_ld32(s_col(t) + lane_base + 96, r1);
-            tmem_wait_ld();
-            if (edge) hide32(r0, lo - 64, hi - 64), hide32(r1, lo - 96, hi - 96);
-            top = fmaxf(top, fmaxf(max32(r0), max32(r1)));
+            if (__any_sync(~0u, lo > 0 || hi < kPTile)) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) hide32(s + 32 * k, lo - 32 * k, hi - 32 * k);
+            }
+            float m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m[k] = max_nan(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
+#pragma unroll
+            for (int k = 8; k < 128; k += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                m[e] = max3_nan(m[e], __uint_as_float(s[k + e]), __uint_as_float(s[k + 4 + e]));
+            const float top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
             // ---- move the reference, and rescale O and the sum, when the maximum outgrew it
             if (__any_sync(~0u, top > ref && (top - ref) * c > 8.0f)) {
               const float to = fmaxf(top, ref);
               const float f = to == -INFINITY ? 1.0f : kv4_exp2((ref - to) * c);
               ref = to;
-              sum *= f;
+              sum2[0] = fma2(sum2[0], pack2(f, f), 0ull);
+              sum2[1] = fma2(sum2[1], pack2(f, f), 0ull);
               if (tile > first) {
-                ok = __all_sync(~0u, ok && mbar_wait(&bars.o_done[t], (o_phase ^ 1u) & 1u));
+                wait(&bars.o_done[t], o_phase ^ 1u);
                 tc_fence_after();
 #pragma unroll 1
-                for (int k = 0; k < D / 32; ++k) {
-                  uint32_t o[32];
-                  tmem_ld32(o_col(t) + lane_base + k * 32, o);
+                for (int k = 0; k < D / 16; ++k) {
+                  uint32_t o[16];
+                  tmem_ld16(o_tm + lane_base + k * 16, o);
                   tmem_wait_ld();
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st32(o_col(t) + lane_base + k * 32, o);
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st16(o_tm + lane_base + k * 16, o);
                 }
                 tmem_wait_st();
               }
             }
-            const float off = ref == -INFINITY ? 0.0f : ref * c;
-            // P (16-bit pairs) over the scores that have been read: columns 0-63 of the tile's S.
-            tmem_ld32(s_col(t) + lane_base, r0);
-            tmem_ld32(s_col(t) + lane_base + 32, r1);
-            tmem_wait_ld();
-            if (edge) hide32(r0, lo, hi), hide32(r1, lo - 32, hi - 32);
-            sum += exp32<T>(r0, c, off, s_col(t) + lane_base);
-            tmem_ld32(s_col(t) + lane_base + 64, r0);
-            sum += exp32<T>(r1, c, off, s_col(t) + lane_base + 16);
-            tmem_ld32(s_col(t) + lane_base + 96, r1);
-            tmem_wait_ld();
-            if (edge) hide32(r0, lo - 64, hi - 64), hide32(r1, lo - 96, hi - 96);
-            sum += exp32<T>(r0, c, off, s_col(t) + lane_base + 32);
-            sum += exp32<T>(r1, c, off, s_col(t) + lane_base + 48);
+            // A NaN or an infinite score makes the whole row NaN, whichever way its column goes.
+            const float off = top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : -ref * c;
+            const uint64_t off2 = pack2(off, off);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // P (16-bit pairs) over columns 0-63 of S
+              exp32<T, kBf16>(s + 32 * k, c2, off2, s_tm + lane_base + 16 * k, sum2);
             tmem_wait_st();
           }
-          o_phase ^= 1u;  // the product of this tile completes phase o_phase ^ 1 of o_done
+          o_phase ^= 1u;  // this step's product completes phase o_phase ^ 1 of o_done
           tc_fence_before();
-          mbar_arrive(&bars.p_full[t]);
+          named_bar_sync(2 + t, 128);
+          if (issuer) {
+            issue_o(it, tile > first);
+            if (tile + 1 < last) issue_s(it + 1);
+          }
         }
-        // ---- O of the piece is complete
-        ok = __all_sync(~0u, ok && mbar_wait(&bars.o_done[t], (o_phase ^ 1u) & 1u));
-        tc_fence_after();
+        float x, y;
+        sum2[0] = add2(sum2[0], sum2[1]);
+        unpack64(sum2[0], x, y);
+        sum = x + y;
+        if (ref == -INFINITY && sum < 1e-30f) sum = 0.0f;  // nothing seen: what is left of 2^-125
+      } else {
+        // The other tile sets the pace: this one counts as having read each step's operands.
+        for (int tile = first; tile < last; ++tile, ++it) {
+          if (!issuer) continue;
+          wait(&bars.k_full[it & 1], it >> 1);
+          if (lane == 0) mbar_arrive(&bars.k_empty[it & 1]);
+          wait(&bars.v_full[it & 1], it >> 1);
+          if (lane == 0) mbar_arrive(&bars.v_empty[it & 1]);
+        }
       }
 
+      // ---- the next item's first scores run while this one is written
       const bool complete = u == w.item && ue == w.item + w.n_tiles;
-      uint16_t* out = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + h) * D;
+      const int fc = complete ? 0 : w.first_cta(), lc = complete ? 0 : w.last_cta();
+      const int side = w.item < w.u0 ? 0 : 1;
+      const bool more = ue < w.u1 && w.next(p);
+      if (more && issuer) begin(w.req.n * p.G - w.rb * kPRows > t * 128);
+
+      if (tile_used) {
+        wait(&bars.o_done[t], o_phase ^ 1u);
+        tc_fence_after();
+      }
       if (complete) {
         if (tile_used) {
           const float inv = sum > 0.0f ? 1.0f / sum : sum;  // nothing seen: zeros; NaN stays
 #pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
-            uint32_t o[32];
-            tmem_ld32(o_col(t) + lane_base + k * 32, o);
+          for (int k = 0; k < D / 64; ++k) {
+            uint32_t o[64];
+            tmem_ld32(o_tm + lane_base + k * 64, o);
+            tmem_ld32(o_tm + lane_base + k * 64 + 32, o + 32);
             tmem_wait_ld();
             if (live) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
+              for (int e = 0; e < 64; e += 8) {
                 uint4 v;
                 v.x = Elem<T>::from_f2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
                 v.y = Elem<T>::from_f2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
                 v.z = Elem<T>::from_f2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
                 v.w = Elem<T>::from_f2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                *reinterpret_cast<uint4*>(out + k * 32 + e) = v;
+                *reinterpret_cast<uint4*>(out + k * 64 + e) = v;
               }
             }
           }
         }
       } else {
         // Part: reference and sum per row, then O as [dims / 4][rows] groups of four.
-        const int fc = w.first_cta(), lc = w.last_cta(), me = (int)blockIdx.x;
-        const int brow = t * 128 + row;
-        float* part = p.partial + (int64_t)(2 * me + (w.item < w.u0 ? 0 : 1)) * slot_floats(D);
+        const int me = (int)blockIdx.x, brow = t * 128 + row;
+        float* part = p.partial + (int64_t)(2 * me + side) * slot_floats(D);
         if (tile_used) {
           part[brow] = ref;
           part[kPRows + brow] = sum;
 #pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
-            uint32_t o[32];
-            tmem_ld32(o_col(t) + lane_base + k * 32, o);
+          for (int k = 0; k < D / 64; ++k) {
+            uint32_t o[64];
+            tmem_ld32(o_tm + lane_base + k * 64, o);
+            tmem_ld32(o_tm + lane_base + k * 64 + 32, o + 32);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(part + 2 * kPRows + ((k * 8 + e / 4) * kPRows + brow) * 4) =
+            for (int e = 0; e < 64; e += 4)
+              *reinterpret_cast<uint4*>(part + 2 * kPRows + ((k * 16 + e / 4) * kPRows + brow) * 4) =
                   make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
@@ -329,27 +446,27 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           const float inv = l > 0.0f ? 1.0f / l : l;
           if (live) {
 #pragma unroll 1
-            for (int k = 0; k < D / 32; ++k) {
-              float v[32];
+            for (int k = 0; k < D / 64; ++k) {
+              float v[64];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+              for (int e = 0; e < 64; ++e) v[e] = 0.0f;
               for (int x = fc; x <= lc; ++x) {
                 const float f = kv4_exp2((__ldcg(slot(x) + brow) - to) * c);
-                const float* src = slot(x) + 2 * kPRows + (k * 8 * kPRows + brow) * 4;
+                const float* src = slot(x) + 2 * kPRows + (k * 16 * kPRows + brow) * 4;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 16; ++e) {
                   const float4 o = __ldcg(reinterpret_cast<const float4*>(src + e * kPRows * 4));
                   v[4 * e] += o.x * f, v[4 * e + 1] += o.y * f, v[4 * e + 2] += o.z * f, v[4 * e + 3] += o.w * f;
                 }
               }
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
+              for (int e = 0; e < 64; e += 8) {
                 uint4 o;
                 o.x = Elem<T>::from_f2(v[e] * inv, v[e + 1] * inv);
                 o.y = Elem<T>::from_f2(v[e + 2] * inv, v[e + 3] * inv);
                 o.z = Elem<T>::from_f2(v[e + 4] * inv, v[e + 5] * inv);
                 o.w = Elem<T>::from_f2(v[e + 6] * inv, v[e + 7] * inv);
-                *reinterpret_cast<uint4*>(out + k * 32 + e) = o;
+                *reinterpret_cast<uint4*>(out + k * 64 + e) = o;
               }
             }
           }
@@ -358,26 +475,38 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       }
       tc_fence_before();
       u = ue;
-      if (u >= w.u1 || !w.next(p)) break;
+      if (!more) break;
     }
-  } else if (warp < 12) {
+  } else {
     // ================================================================ codes to operands
     const int dw = warp - 8, key = tid - 256;
     const int vr = (lane >> 1) & 1, vh = lane & 1, vg = lane >> 2;  // values: record, token half, dim group
     const int rpb = p.c.P / kKv4Rec;
+    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale goes into Q
     uint32_t it = 0;
     bool ok = true;
     uint32_t kc[4 * NW], kp[NG], vq[NG], vc[4 * NW], vp[8 * NG];
-    const uint8_t *ra, *rb;  // this warp's two records of a tile
     for (long long u = w.u0; u < w.u1 && ok;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
       const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
       const int* table = p.table + (int64_t)w.r * p.table_stride;
       const int n_rec = (w.req.len + kKv4Rec - 1) / kKv4Rec;
-      const auto records = [&](int tile) {
-        ra = kv4_record(p, table, tile * 8 + 2 * dw, n_rec, rpb, w.kvh, REC);
-        rb = kv4_record(p, table, tile * 8 + 2 * dw + 1, n_rec, rpb, w.kvh, REC);
+      // This warp's two records of a tile: their blocks are looked up one tile before their codes
+      // are loaded, which is one tile before they are unpacked.
+      const auto block_of = [&](int rec) {
+        if (rec >= n_rec) return -1;
+        const int b = __ldg(table + (int)((uint32_t)rec / (uint32_t)rpb));
+        if (b >= 0 && b < p.c.n_blocks) return b;
+        record_status(FQKV_STATUS_BAD_INDEX);
+        return 0;
       };
+      const auto address = [&](int rec, int block) -> const uint8_t* {
+        if (block < 0) return nullptr;
+        return p.c.data + (((int64_t)block * p.c.n_kv + w.kvh) * rpb + (int)((uint32_t)rec % (uint32_t)rpb)) * REC;
+      };
+      const uint8_t *ra = address(first * 8 + 2 * dw, block_of(first * 8 + 2 * dw)),
+                    *rb = address(first * 8 + 2 * dw + 1, block_of(first * 8 + 2 * dw + 1));
+      int next_a = block_of(first * 8 + 8 + 2 * dw), next_b = block_of(first * 8 + 8 + 2 * dw + 1);
       // Codes and parameters of this thread's key; a key past the last one gets zeros.
       const auto load_k = [&](int tile) {
         const uint8_t* rec = lane < 16 ? ra : rb;
@@ -417,15 +546,40 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
                       ? __ldg(reinterpret_cast<const uint32_t*>(rec + 16 * D + 64 * NG) + 8 * NG * vh + k)
                       : 0u;
       };
-      records(first);
       load_k(first);
       load_v(first);
+      // ---- the item's queries, once the previous item's last scores have been formed
+      if (it > 0) ok = mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
+      constexpr int CH = D / 8, BATCH = 8;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kPRows * CH / 128; k0 += BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int row = (k0 + k) * (128 / CH) + key / CH, grow = w.rb * kPRows + row;
+          const int j = (int)((uint32_t)grow / (uint32_t)p.G), h = grow - j * p.G;
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (j < w.req.n)
+            v[k] = *reinterpret_cast<const uint4*>(
+                p.q + (p.query_start ? (int64_t)(w.req.start + j) * p.q_t : w.r * p.q_r + j * p.q_t) +
+                (int64_t)(w.kvh * p.G + h) * p.q_h + key % CH * 8);
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int row = (k0 + k) * (128 / CH) + key / CH, ch = key % CH;
+          v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
+          *reinterpret_cast<uint4*>(smem + (row / 128) * OP + (ch / 8) * 128 * 128 + sw128_offset(row % 128, ch % 8)) =
+              v[k];
+        }
+      }
+      fence_proxy_async_smem();
+      warp_arrive(&bars.q_full);
       for (int tile = first; tile < last && ok; ++tile, ++it) {
         const int stage = it & 1;
         const uint32_t phase = (it >> 1) & 1u;
         uint8_t* k_tile = smem + (2 + stage) * OP;
         uint8_t* v_tile = smem + (4 + stage) * OP;
-        if (it >= 2) ok = mbar_wait(&bars.k_empty[stage], phase ^ 1u);
+        if (it >= 2) ok = ok && mbar_wait(&bars.k_empty[stage], phase ^ 1u);
         // ---- keys: a word is eight dims, one 16-byte chunk of the key's row
         uint32_t hide = 0;  // a key whose value row is NaN scores NaN, so whoever sees it becomes NaN
 #pragma unroll
@@ -449,10 +603,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           }
         }
         fence_proxy_async_smem();
-        mbar_arrive(&bars.k_full[stage]);
+        warp_arrive(&bars.k_full[stage]);
         if (tile + 1 < last) {
-          records(tile + 1);
+          ra = address(tile * 8 + 8 + 2 * dw, next_a);
+          rb = address(tile * 8 + 8 + 2 * dw + 1, next_b);
           load_k(tile + 1);
+          next_a = block_of(tile * 8 + 16 + 2 * dw);
+          next_b = block_of(tile * 8 + 16 + 2 * dw + 1);
         }
         if (it >= 2) ok = ok && mbar_wait(&bars.v_empty[stage], phase ^ 1u);
         // ---- values: rows are dims, a chunk is eight tokens
@@ -490,75 +647,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           }
         }
         fence_proxy_async_smem();
-        mbar_arrive(&bars.v_full[stage]);
+        warp_arrive(&bars.v_full[stage]);
         if (tile + 1 < last) load_v(tile + 1);
       }
       u = ue;
       if (u >= w.u1 || !w.next(p)) break;
     }
-  } else {
-    if (lane == 0) {
-      // ============================================================== products
-      constexpr uint32_t idesc_s = make_idesc_f16(128, 128, kBf16), idesc_o = make_idesc_f16(128, D, kBf16);
-      const uint32_t base = smem_u32(smem);
-      uint32_t it = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-      bool ok = true;
-      const auto issue_s = [&](int t, int stage) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * 128 * 128 + (k % 4) * 32;
-          umma_f16(s_col(t), make_sw128_desc(base + t * OP + off), make_sw128_desc(base + (2 + stage) * OP + off),
-                   idesc_s, k > 0);
-        }
-        umma_commit(&bars.s_full[t]);
-      };
-      const auto issue_o = [&](int t, int stage, bool accumulate) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_ts(o_col(t), s_col(t) + k * 8,
-                      make_sw128_desc(base + (4 + stage) * OP + (k / 4) * D * 128 + (k % 4) * 32), idesc_o,
-                      accumulate || k > 0);
-        umma_commit(&bars.o_done[t]);
-      };
-      for (long long u = w.u0; u < w.u1 && ok;) {
-        const long long ue = min(w.u1, w.item + w.n_tiles);
-        const int n = (int)(ue - u);
-        const int tiles = w.req.n * p.G - w.rb * kPRows > 128 ? 2 : 1;
-        for (int x = 0; x <= n && ok; ++x) {
-          // Step x: the second products of tile x - 1, then the first products of tile x.
-          const uint32_t a = it + x, b = it + x - 1;
-          if (x < n) ok = ok && mbar_wait(&bars.k_full[a & 1], (a >> 1) & 1u);
-          if (x > 0) ok = ok && mbar_wait(&bars.v_full[b & 1], (b >> 1) & 1u);
-          for (int t = 0; t < tiles && ok; ++t) {
-            if (x == 0) {
-              ok = ok && mbar_wait(&bars.q_full[t], q_phase[t]);
-              q_phase[t] ^= 1u;
-            } else {
-              ok = ok && mbar_wait(&bars.p_full[t], p_phase[t]);
-              p_phase[t] ^= 1u;
-            }
-            tc_fence_after();
-            if (!ok) break;
-            if (x > 0) issue_o(t, b & 1, x > 1);
-            if (x < n) issue_s(t, a & 1);
-          }
-          if (x < n) umma_commit(&bars.k_empty[a & 1]);
-          if (x > 0) umma_commit(&bars.v_empty[b & 1]);
-        }
-        it += n;
-        u = ue;
-        if (u >= w.u1 || !w.next(p)) break;
-      }
-      // Everything issued has completed before TMEM is freed.
-      mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
-      mbar_wait(&bars.v_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
-    }
-    __syncwarp();
   }
+  // Every product has completed: each tile's last O was waited for, and its scores come before it.
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int D, int NG>
