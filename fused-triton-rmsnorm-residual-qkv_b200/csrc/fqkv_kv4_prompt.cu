@@ -136,6 +136,9 @@ __device__ __forceinline__ void hide32(uint32_t* r, int lo, int hi) {
     if (k < lo || k >= hi) r[k] = 0xFF800000u;
 }
 // P = exp2(c S - off) of 32 keys to 16 columns at `dst`, added to `sum` in fp32.
+#ifndef POLY
+#define POLY 0x88
+#endif
 template <typename T, bool BF16>
 __device__ __forceinline__ void exp32(const uint32_t* r, uint64_t c, uint64_t off, uint32_t dst, uint64_t (&sum)[2]) {
   uint32_t pk[16];
@@ -143,7 +146,7 @@ __device__ __forceinline__ void exp32(const uint32_t* r, uint64_t c, uint64_t of
   for (int k = 0; k < 16; ++k) {
     uint64_t x = fma2(pack2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), c, off);
     float a, b;
-    if (k % 4 == 3) {
+    if (POLY >> (k % 8) & 1) {
       x = exp2_poly2<BF16>(x);
       unpack64(x, a, b);
     } else {
@@ -162,6 +165,10 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
+}
+// Asynchronous 16-byte copy global -> shared; zeros where `in` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 // One arrival for a warp whose lanes have all got here.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     const int dw = warp - 8, key = tid - 256;
     const int vr = (lane >> 1) & 1, vh = lane & 1, vg = lane >> 2;  // values: record, token half, dim group
     const int rpb = p.c.P / kKv4Rec;
-    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale goes into Q
+    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale negates the keys
     uint32_t it = 0;
     bool ok = true;
     uint32_t kc[4 * NW], kp[NG], vq[NG], vc[4 * NW], vp[8 * NG];
@@ -491,22 +498,39 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
       const int* table = p.table + (int64_t)w.r * p.table_stride;
       const int n_rec = (w.req.len + kKv4Rec - 1) / kKv4Rec;
-      // This warp's two records of a tile: their blocks are looked up one tile before their codes
-      // are loaded, which is one tile before they are unpacked.
-      const auto block_of = [&](int rec) {
-        if (rec >= n_rec) return -1;
-        const int b = __ldg(table + (int)((uint32_t)rec / (uint32_t)rpb));
-        if (b >= 0 && b < p.c.n_blocks) return b;
-        record_status(FQKV_STATUS_BAD_INDEX);
-        return 0;
+      // This warp's two records of a tile: (nth, off) are the block's place in the table and the
+      // record's in the block, stepped without a division.  Blocks are looked up one tile before
+      // their codes are loaded, which is one tile before they are unpacked.
+      const int step_n = 8 / rpb, step_o = 8 % rpb;
+      int nth[2], off[2], ahead = first * 8 + 2 * dw, next[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        nth[k] = (int)((uint32_t)(ahead + k) / (uint32_t)rpb);
+        off[k] = ahead + k - nth[k] * rpb;
+        next[k] = ahead + k < n_rec ? __ldg(table + nth[k]) : -1;
+      }
+      const uint8_t *ra, *rb;
+      const auto advance = [&]() {  // ra, rb: the records of the tile `ahead`; then the next tile's blocks
+        const uint8_t* at[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          at[k] = nullptr;
+          if (ahead + k < n_rec) {
+            if (next[k] < 0 || next[k] >= p.c.n_blocks) {
+              record_status(FQKV_STATUS_BAD_INDEX);
+              next[k] = 0;
+            }
+            at[k] = p.c.data + (((int64_t)next[k] * p.c.n_kv + w.kvh) * rpb + off[k]) * REC;
+          }
+          nth[k] += step_n;
+          off[k] += step_o;
+          if (off[k] >= rpb) off[k] -= rpb, ++nth[k];
+          next[k] = ahead + 8 + k < n_rec ? __ldg(table + nth[k]) : -1;
+        }
+        ra = at[0], rb = at[1];
+        ahead += 8;
       };
-      const auto address = [&](int rec, int block) -> const uint8_t* {
-        if (block < 0) return nullptr;
-        return p.c.data + (((int64_t)block * p.c.n_kv + w.kvh) * rpb + (int)((uint32_t)rec % (uint32_t)rpb)) * REC;
-      };
-      const uint8_t *ra = address(first * 8 + 2 * dw, block_of(first * 8 + 2 * dw)),
-                    *rb = address(first * 8 + 2 * dw + 1, block_of(first * 8 + 2 * dw + 1));
-      int next_a = block_of(first * 8 + 8 + 2 * dw), next_b = block_of(first * 8 + 8 + 2 * dw + 1);
+      advance();
       // Codes and parameters of this thread's key; a key past the last one gets zeros.
       const auto load_k = [&](int tile) {
         const uint8_t* rec = lane < 16 ? ra : rb;
@@ -550,27 +574,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       load_v(first);
       // ---- the item's queries, once the previous item's last scores have been formed
       if (it > 0) ok = mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
-      constexpr int CH = D / 8, BATCH = 8;
-#pragma unroll 1
-      for (int k0 = 0; k0 < kPRows * CH / 128; k0 += BATCH) {
-        uint4 v[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int row = (k0 + k) * (128 / CH) + key / CH, grow = w.rb * kPRows + row;
-          const int j = (int)((uint32_t)grow / (uint32_t)p.G), h = grow - j * p.G;
-          v[k] = make_uint4(0, 0, 0, 0);
-          if (j < w.req.n)
-            v[k] = *reinterpret_cast<const uint4*>(
-                p.q + (p.query_start ? (int64_t)(w.req.start + j) * p.q_t : w.r * p.q_r + j * p.q_t) +
-                (int64_t)(w.kvh * p.G + h) * p.q_h + key % CH * 8);
+      constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row; rows copied at a time
+      {
+        const int ch = key % CH, dj = STEP / p.G, dh = STEP % p.G;
+        int row = key / CH, j = (int)((uint32_t)(w.rb * kPRows + row) / (uint32_t)p.G);
+        int h = w.rb * kPRows + row - j * p.G;
+        const uint16_t* q0 = p.q + (p.query_start ? (int64_t)w.req.start * p.q_t : w.r * p.q_r) +
+                             (int64_t)(w.kvh * p.G) * p.q_h + ch * 8;
+#pragma unroll 4
+        for (; row < kPRows; row += STEP) {
+          const bool in = j < w.req.n;
+          const uint16_t* src = in ? q0 + j * p.q_t + h * p.q_h : p.q;
+          copy16(smem_u32(smem) + (row / 128) * OP + (ch / 8) * 128 * 128 + sw128_offset(row % 128, ch % 8), src, in);
+          j += dj;
+          h += dh;
+          if (h >= p.G) h -= p.G, ++j;
         }
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int row = (k0 + k) * (128 / CH) + key / CH, ch = key % CH;
-          v[k].x ^= flip, v[k].y ^= flip, v[k].z ^= flip, v[k].w ^= flip;
-          *reinterpret_cast<uint4*>(smem + (row / 128) * OP + (ch / 8) * 128 * 128 + sw128_offset(row % 128, ch % 8)) =
-              v[k];
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
       }
       fence_proxy_async_smem();
       warp_arrive(&bars.q_full);
@@ -581,23 +601,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         uint8_t* v_tile = smem + (4 + stage) * OP;
         if (it >= 2) ok = ok && mbar_wait(&bars.k_empty[stage], phase ^ 1u);
         // ---- keys: a word is eight dims, one 16-byte chunk of the key's row
-        uint32_t hide = 0;  // a key whose value row is NaN scores NaN, so whoever sees it becomes NaN
+        uint32_t hide = flip;  // a key whose value row is NaN scores NaN, so whoever sees it becomes NaN
 #pragma unroll
         for (int k = 0; k < NG; ++k)
-          if (not_finite<kBf16>(vq[k])) hide = 0x7FFF7FFFu;
+          if (not_finite<kBf16>(vq[k])) hide = 0xFFFFFFFFu;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          const uint32_t par = kp[i * NG / NW];
+          const uint32_t par = hide == 0xFFFFFFFFu ? hide : kp[i * NG / NW] ^ hide;
           const uint32_t s2 = __byte_perm(par, par, 0x1010), m2 = __byte_perm(par, par, 0x3232);
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
             const uint32_t x = kc[cc * NW + i];  // dims 32 i + 8 cc ..
             using N = Kv4Nib<T>;
             uint4 v;
-            v.x = N::fma2(N::sub2(N::template pair<0>(x), N::kOffset2), s2, m2) | hide;
-            v.y = N::fma2(N::sub2(N::template pair<1>(x), N::kOffset2), s2, m2) | hide;
-            v.z = N::fma2(N::sub2(N::template pair<2>(x), N::kOffset2), s2, m2) | hide;
-            v.w = N::fma2(N::sub2(N::template pair<3>(x), N::kOffset2), s2, m2) | hide;
+            v.x = N::fma2(N::sub2(N::template pair<0>(x), N::kOffset2), s2, m2);
+            v.y = N::fma2(N::sub2(N::template pair<1>(x), N::kOffset2), s2, m2);
+            v.z = N::fma2(N::sub2(N::template pair<2>(x), N::kOffset2), s2, m2);
+            v.w = N::fma2(N::sub2(N::template pair<3>(x), N::kOffset2), s2, m2);
             const int chunk = 4 * i + cc;
             *reinterpret_cast<uint4*>(k_tile + (chunk / 8) * 128 * 128 + sw128_offset(key, chunk % 8)) = v;
           }
@@ -605,11 +625,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         fence_proxy_async_smem();
         warp_arrive(&bars.k_full[stage]);
         if (tile + 1 < last) {
-          ra = address(tile * 8 + 8 + 2 * dw, next_a);
-          rb = address(tile * 8 + 8 + 2 * dw + 1, next_b);
+          advance();
           load_k(tile + 1);
-          next_a = block_of(tile * 8 + 16 + 2 * dw);
-          next_b = block_of(tile * 8 + 16 + 2 * dw + 1);
         }
         if (it >= 2) ok = ok && mbar_wait(&bars.v_empty[stage], phase ^ 1u);
         // ---- values: rows are dims, a chunk is eight tokens
