@@ -11,24 +11,25 @@
 // Shape.  A CTA takes 256 query rows of one KV head (all heads that share it, so the keys are
 // unpacked once for them) as two tiles of 128 and walks the keys 128 at a time:
 //   warps 0-3, 4-7   softmax of the two tiles, one row per thread, S and O in TMEM; P goes back
-//                    to TMEM over S and is the A operand of the second product.  The first warp
-//                    of each issues its tile's products, P V(j) and then S(j+1), so one tile's
-//                    softmax runs under the other tile's products
+//                    to TMEM over S and is the A operand of the second product
 //   warps 8-11       4-bit codes from global memory to swizzled shared-memory operands, and the
 //                    queries of the next item while the current one ends
-// Twelve warps leave a thread 168 registers: a row's 128 scores are read from TMEM once.
+//   warp 12          issues the products
+// TMEM holds two O tiles and two S tiles, so a step's 128 keys are taken as two halves: while a
+// tile's warps exponentiate one half, the tensor core forms the scores of the other (and works for
+// the other tile).  S of a half follows P V of the same half, in issue order, into the same columns.
 // The values are stored transposed (dims x keys, K-major) because the cache interleaves tokens
 // in pairs: a thread's eight tokens of one dim are one 16-byte store without any permutation.
 //
-// Bound: per 128 keys the four products take 2048 tensor cycles and the softmax 32768
-// exponentials, 2048 cycles of the special function unit: a quarter of them is a polynomial
-// on the FMA pipe instead (packed pairs), the scaling and the sums are packed pairs too.
+// Bound: per 128 keys the products take 2048 tensor cycles at full rate, the softmax 32768
+// exponentials (2048 cycles of the special function unit) and the unpacking about 500 issue slots
+// of every scheduler.
 #include "fqkv_kv4_work.cuh"
 
 namespace fqkv {
 namespace {
 
-constexpr int kPThreads = 384;
+constexpr int kPThreads = 416;
 constexpr int kPRows = 256;
 constexpr int kPTile = 128;  // keys per step
 constexpr int kPMinTiles = 4;
@@ -99,36 +100,6 @@ __device__ __forceinline__ float max3_nan(float x, float y, float z) {
   return r;
 }
 
-// 2^x for a pair, x < 127, on the FMA pipe: x = i + f with i the nearest integer,
-// 2^f by a polynomial (largest relative error 7.5e-5 at degree 3, for P rounded to bf16, 2.6e-6 at
-// degree 4 for fp16; fitted by equalising the error's extremes on [-1/2, 1/2]), i added to the
-// exponent.  Below 2^-125 the result is 2^-125, which is zero beside a row's largest entry.
-template <bool BF16>
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-  float a, b;
-  unpack64(x, a, b);
-  x = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
-  const uint64_t magic = pack2(12582912.0f, 12582912.0f), minus = pack2(-12582912.0f, -12582912.0f);
-  const uint64_t t = add2(x, magic);  // the integer in the low mantissa bits
-  const uint64_t f = fma2(add2(t, minus), pack2(-1.0f, -1.0f), x);
-  uint64_t r;
-  if constexpr (BF16) {
-    r = fma2(f, pack2(0.05517166852951f, 0.05517166852951f), pack2(0.24261112511158f, 0.24261112511158f));
-    r = fma2(r, f, pack2(0.69326096773148f, 0.69326096773148f));
-    r = fma2(r, f, pack2(0.99992805719376f, 0.99992805719376f));
-  } else {
-    r = fma2(f, pack2(0.00957010220736f, 0.00957010220736f), pack2(0.05591785907745f, 0.05591785907745f));
-    r = fma2(r, f, pack2(0.24024744331837f, 0.24024744331837f));
-    r = fma2(r, f, pack2(0.69312179088593f, 0.69312179088593f));
-    r = fma2(r, f, pack2(0.99999928474426f, 0.99999928474426f));
-  }
-  float ta, tb;
-  unpack64(t, ta, tb);
-  unpack64(r, a, b);
-  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
-               __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
-}
-
 // Scores of keys outside [lo, hi) of a chunk become -inf.
 __device__ __forceinline__ void hide32(uint32_t* r, int lo, int hi) {
 #pragma unroll
@@ -136,26 +107,17 @@ __device__ __forceinline__ void hide32(uint32_t* r, int lo, int hi) {
     if (k < lo || k >= hi) r[k] = 0xFF800000u;
 }
 // P = exp2(c S - off) of 32 keys to 16 columns at `dst`, added to `sum` in fp32.
-#ifndef POLY
-#define POLY 0x88
-#endif
-template <typename T, bool BF16>
+template <typename T>
 __device__ __forceinline__ void exp32(const uint32_t* r, uint64_t c, uint64_t off, uint32_t dst, uint64_t (&sum)[2]) {
   uint32_t pk[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    uint64_t x = fma2(pack2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), c, off);
+    const uint64_t x = fma2(pack2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), c, off);
     float a, b;
-    if (POLY >> (k % 8) & 1) {
-      x = exp2_poly2<BF16>(x);
-      unpack64(x, a, b);
-    } else {
-      unpack64(x, a, b);
-      a = kv4_exp2(a);
-      b = kv4_exp2(b);
-      x = pack2(a, b);
-    }
-    sum[k & 1] = add2(sum[k & 1], x);
+    unpack64(x, a, b);
+    a = kv4_exp2(a);
+    b = kv4_exp2(b);
+    sum[k & 1] = add2(sum[k & 1], pack2(a, b));
     pk[k] = Elem<T>::from_f2(a, b);
   }
   tmem_st16(dst, pk);
@@ -178,9 +140,10 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 
 struct Bars {
   uint64_t k_full[2], v_full[2];    // operands of a step written: one arrival per unpacking warp
-  uint64_t k_empty[2], v_empty[2];  // and read by both tiles' products
+  uint64_t k_empty[2], v_empty[2];  // and read by all products
   uint64_t q_full;                  // the queries of an item
-  uint64_t s_full[2], o_done[2];    // a tile's scores; its part of O
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][half]: scores formed; probabilities written
+  uint64_t o_done[2];                   // a half's part of O added
 };
 
 // Whether a scale or a minimum (packed pair) is a NaN or an infinity.
@@ -218,10 +181,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.k_full[i], 4);
       mbar_init(&bars.v_full[i], 4);
-      mbar_init(&bars.k_empty[i], 2);
-      mbar_init(&bars.v_empty[i], 2);
-      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
       mbar_init(&bars.o_done[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars.s_full[i][h], 1);
+        mbar_init(&bars.p_full[i][h], 4);
+      }
     }
     mbar_init(&bars.q_full, 4);
     fence_mbarrier_init_cluster();
@@ -240,54 +206,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
   const uint32_t tmem = s_tmem;
 
   if (warp < 8) {
-    // ================================================================ softmax and products
+    // ================================================================ softmax
     const int t = warp >> 2, row = tid & 127;  // tile, row of the tile = TMEM lane
-    const uint32_t s_tm = tmem + t * 128, o_tm = tmem + 256 + t * 128;  // S (P over it), O
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const bool issuer = (warp & 3) == 0;
+    const uint32_t s_tm = tmem + t * 128 + lane_base, o_tm = tmem + 256 + t * 128 + lane_base;  // S (P over it), O
     const float c = fabsf(p.scale_log2);
     const uint64_t c2 = pack2(c, c);
-    constexpr uint32_t idesc_s = make_idesc_f16(128, 128, kBf16), idesc_o = make_idesc_f16(128, D, kBf16);
-    // Descriptors are one 64-bit base and constant steps (16-byte units).
-    const uint64_t base = make_sw128_desc(smem_u32(smem));
-    uint32_t it = 0, s_phase = 0, o_phase = 0, q_phase = 0;
+    uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;  // after a wait that ran out nothing is waited for, and every barrier is still reached
     const auto wait = [&](uint64_t* bar, uint32_t phase) { ok = __all_sync(~0u, ok && mbar_wait(bar, phase & 1u)); };
-    // Scores of step x (the issuing warp).
-    const auto issue_s = [&](uint32_t x) {
-      wait(&bars.k_full[x & 1], x >> 1);
-      tc_fence_after();
-      const uint64_t a = base + (uint64_t)(t * (OP >> 4)), b = base + (uint64_t)((2 + (x & 1)) * (OP >> 4));
-      if (elect_one()) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = ((k / 4) * 128 * 128 + (k % 4) * 32) >> 4;
-          umma_f16(s_tm, a + off, b + off, idesc_s, k > 0);
-        }
-        umma_commit(&bars.s_full[t]);
-        umma_commit(&bars.k_empty[x & 1]);
-      }
-      __syncwarp();
-    };
-    const auto issue_o = [&](uint32_t x, bool accumulate) {
-      wait(&bars.v_full[x & 1], x >> 1);
-      tc_fence_after();
-      const uint64_t b = base + (uint64_t)((4 + (x & 1)) * (OP >> 4));
-      if (elect_one()) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_ts(o_tm, s_tm + k * 8, b + (((k / 4) * D * 128 + (k % 4) * 32) >> 4), idesc_o, k > 0 || accumulate);
-        umma_commit(&bars.o_done[t]);
-        umma_commit(&bars.v_empty[x & 1]);
-      }
-      __syncwarp();
-    };
-    // First scores of the item (the issuing warp); a tile without rows only lets its steps pass.
-    const auto begin = [&](bool used) {
-      wait(&bars.q_full, q_phase);
-      if (used) issue_s(it);
-    };
-    if (issuer) begin(w.req.n * p.G - w.rb * kPRows > t * 128);
     for (long long u = w.u0; u < w.u1;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
       const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
@@ -298,97 +225,85 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       const bool tile_used = rows > t * 128;
       uint16_t* out = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + grow - j * p.G) * D;
       float ref = -INFINITY, sum = 0.0f;
-      q_phase ^= 1u;
       if (tile_used) {
         const int pos = w.req.len - w.req.n + j;
         const int see_hi = live ? min(pos + 1, w.req.len) : w.req.len;      // keys [see_lo, see_hi)
         const int see_lo = live && p.window > 0 ? max(0, pos - p.window + 1) : 0;
         const bool warp_live = rows > t * 128 + (warp & 3) * 32;
         uint64_t sum2[2] = {0, 0};
-        for (int tile = first; tile < last; ++tile, ++it) {
-          wait(&bars.s_full[t], s_phase);
-          s_phase ^= 1u;
-          tc_fence_after();
-          if (warp_live) {
-            uint32_t s[128];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tmem_ld32(s_tm + lane_base + 32 * k, s + 32 * k);
-            tmem_wait_ld();
-            const int lo = see_lo - tile * kPTile, hi = see_hi - tile * kPTile;
-            if (__any_sync(~0u, lo > 0 || hi < kPTile)) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) hide32(s + 32 * k, lo - 32 * k, hi - 32 * k);
-            }
-            float m[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m[k] = max_nan(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
-#pragma unroll
-            for (int k = 8; k < 128; k += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                m[e] = max3_nan(m[e], __uint_as_float(s[k + e]), __uint_as_float(s[k + 4 + e]));
-            const float top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
-            // ---- move the reference, and rescale O and the sum, when the maximum outgrew it
-            if (__any_sync(~0u, top > ref && (top - ref) * c > 8.0f)) {
-              const float to = fmaxf(top, ref);
-              const float f = to == -INFINITY ? 1.0f : kv4_exp2((ref - to) * c);
-              ref = to;
-              sum2[0] = fma2(sum2[0], pack2(f, f), 0ull);
-              sum2[1] = fma2(sum2[1], pack2(f, f), 0ull);
-              if (tile > first) {
-                wait(&bars.o_done[t], o_phase ^ 1u);
-                tc_fence_after();
+        for (int tile = first; tile < last; ++tile) {
 #pragma unroll 1
-                for (int k = 0; k < D / 16; ++k) {
-                  uint32_t o[16];
-                  tmem_ld16(o_tm + lane_base + k * 16, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st16(o_tm + lane_base + k * 16, o);
-                }
-                tmem_wait_st();
+          for (int half = 0; half < 2; ++half) {
+            wait(&bars.s_full[t][half], s_phase);
+            tc_fence_after();
+            if (warp_live) {
+              uint32_t s[64];
+              const uint32_t at = s_tm + half * 64;
+              tmem_ld32(at, s);
+              tmem_ld32(at + 32, s + 32);
+              tmem_wait_ld();
+              const int key0 = tile * kPTile + half * 64, lo = see_lo - key0, hi = see_hi - key0;
+              if (__any_sync(~0u, lo > 0 || hi < 64)) {
+                hide32(s, lo, hi);
+                hide32(s + 32, lo - 32, hi - 32);
               }
-            }
-            // A NaN or an infinite score makes the whole row NaN, whichever way its column goes.
-            const float off = top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : -ref * c;
-            const uint64_t off2 = pack2(off, off);
+              float m[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)  // P (16-bit pairs) over columns 0-63 of S
-              exp32<T, kBf16>(s + 32 * k, c2, off2, s_tm + lane_base + 16 * k, sum2);
-            tmem_wait_st();
+              for (int k = 0; k < 4; ++k) m[k] = max_nan(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
+#pragma unroll
+              for (int k = 8; k < 64; k += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  m[e] = max3_nan(m[e], __uint_as_float(s[k + e]), __uint_as_float(s[k + 4 + e]));
+              const float top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+              // ---- move the reference, and rescale O and the sum, when the maximum outgrew it
+              if (__any_sync(~0u, top > ref && (top - ref) * c > 8.0f)) {
+                const float to = fmaxf(top, ref);
+                const float f = to == -INFINITY ? 1.0f : kv4_exp2((ref - to) * c);
+                ref = to;
+                sum2[0] = fma2(sum2[0], pack2(f, f), 0ull);
+                sum2[1] = fma2(sum2[1], pack2(f, f), 0ull);
+                if (tile > first || half) {
+                  wait(&bars.o_done[t], o_phase ^ 1u);
+                  tc_fence_after();
+#pragma unroll 1
+                  for (int k = 0; k < D / 16; ++k) {
+                    uint32_t o[16];
+                    tmem_ld16(o_tm + k * 16, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st16(o_tm + k * 16, o);
+                  }
+                  tmem_wait_st();
+                }
+              }
+              // A NaN or an infinite score makes the whole row NaN.
+              const float off = top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : -ref * c;
+              const uint64_t off2 = pack2(off, off);
+              exp32<T>(s, c2, off2, at, sum2);  // P (16-bit pairs) over the half's first 32 columns
+              exp32<T>(s + 32, c2, off2, at + 16, sum2);
+              tmem_wait_st();
+            }
+            // A half's scores say that the product two halves ago is done: before the last half is let
+            // go, the one before it is waited for, so that the wait for the last cannot mistake them.
+            if (half && tile + 1 == last) wait(&bars.o_done[t], o_phase ^ 1u);
+            o_phase ^= 1u;  // this half's product completes phase o_phase ^ 1 of o_done
+            tc_fence_before();
+            warp_arrive(&bars.p_full[t][half]);
           }
-          o_phase ^= 1u;  // this step's product completes phase o_phase ^ 1 of o_done
-          tc_fence_before();
-          named_bar_sync(2 + t, 128);
-          if (issuer) {
-            issue_o(it, tile > first);
-            if (tile + 1 < last) issue_s(it + 1);
-          }
+          s_phase ^= 1u;
         }
         float x, y;
         sum2[0] = add2(sum2[0], sum2[1]);
         unpack64(sum2[0], x, y);
         sum = x + y;
-        if (ref == -INFINITY && sum < 1e-30f) sum = 0.0f;  // nothing seen: what is left of 2^-125
-      } else {
-        // The other tile sets the pace: this one counts as having read each step's operands.
-        for (int tile = first; tile < last; ++tile, ++it) {
-          if (!issuer) continue;
-          wait(&bars.k_full[it & 1], it >> 1);
-          if (lane == 0) mbar_arrive(&bars.k_empty[it & 1]);
-          wait(&bars.v_full[it & 1], it >> 1);
-          if (lane == 0) mbar_arrive(&bars.v_empty[it & 1]);
-        }
       }
 
-      // ---- the next item's first scores run while this one is written
       const bool complete = u == w.item && ue == w.item + w.n_tiles;
       const int fc = complete ? 0 : w.first_cta(), lc = complete ? 0 : w.last_cta();
       const int side = w.item < w.u0 ? 0 : 1;
       const bool more = ue < w.u1 && w.next(p);
-      if (more && issuer) begin(w.req.n * p.G - w.rb * kPRows > t * 128);
-
       if (tile_used) {
         wait(&bars.o_done[t], o_phase ^ 1u);
         tc_fence_after();
@@ -399,8 +314,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
 #pragma unroll 1
           for (int k = 0; k < D / 64; ++k) {
             uint32_t o[64];
-            tmem_ld32(o_tm + lane_base + k * 64, o);
-            tmem_ld32(o_tm + lane_base + k * 64 + 32, o + 32);
+            tmem_ld32(o_tm + k * 64, o);
+            tmem_ld32(o_tm + k * 64 + 32, o + 32);
             tmem_wait_ld();
             if (live) {
 #pragma unroll
@@ -425,8 +340,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
 #pragma unroll 1
           for (int k = 0; k < D / 64; ++k) {
             uint32_t o[64];
-            tmem_ld32(o_tm + lane_base + k * 64, o);
-            tmem_ld32(o_tm + lane_base + k * 64 + 32, o + 32);
+            tmem_ld32(o_tm + k * 64, o);
+            tmem_ld32(o_tm + k * 64 + 32, o + 32);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 64; e += 4)
@@ -484,7 +399,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       u = ue;
       if (!more) break;
     }
-  } else {
+  } else if (warp < 12) {
     // ================================================================ codes to operands
     const int dw = warp - 8, key = tid - 256;
     const int vr = (lane >> 1) & 1, vh = lane & 1, vg = lane >> 2;  // values: record, token half, dim group
@@ -666,6 +581,77 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         fence_proxy_async_smem();
         warp_arrive(&bars.v_full[stage]);
         if (tile + 1 < last) load_v(tile + 1);
+      }
+      u = ue;
+      if (u >= w.u1 || !w.next(p)) break;
+    }
+  } else {
+    // ================================================================ products
+    constexpr uint32_t idesc_s = make_idesc_f16(128, 64, kBf16), idesc_o = make_idesc_f16(128, D, kBf16);
+    // Descriptors are one 64-bit base and constant steps (16-byte units).  The whole warp walks the
+    // loop, so that the addresses stay warp-uniform, and one elected lane issues.
+    const uint64_t base = make_sw128_desc(smem_u32(smem));
+    uint32_t it = 0, q_phase = 0, p_phase[2] = {0, 0};
+    bool ok = true;
+    const auto wait = [&](uint64_t* bar, uint32_t phase) { ok = __all_sync(~0u, ok && mbar_wait(bar, phase & 1u)); };
+    const auto issue_s = [&](int t, int h, uint32_t x) {
+      const uint64_t a = base + (uint64_t)(t * (OP >> 4)),
+                     b = base + (uint64_t)((2 + (x & 1)) * (OP >> 4) + h * (64 * 128 >> 4));
+      const uint32_t d = tmem + t * 128 + h * 64;
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = ((k / 4) * 128 * 128 + (k % 4) * 32) >> 4;
+          umma_f16(d, a + off, b + off, idesc_s, k > 0);
+        }
+        umma_commit(&bars.s_full[t][h]);
+      }
+      __syncwarp();
+    };
+    const auto issue_o = [&](int t, int h, uint32_t x, bool accumulate) {
+      const uint64_t b = base + (uint64_t)((4 + (x & 1)) * (OP >> 4) + h * (D * 128 >> 4));
+      const uint32_t a = tmem + t * 128 + h * 64, d = tmem + 256 + t * 128;
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f16_ts(d, a + k * 8, b + (k * 32 >> 4), idesc_o, k > 0 || accumulate);
+        umma_commit(&bars.o_done[t]);
+      }
+      __syncwarp();
+    };
+    const auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    for (long long u = w.u0; u < w.u1 && ok;) {
+      const long long ue = min(w.u1, w.item + w.n_tiles);
+      const int n = (int)(ue - u), tiles = w.req.n * p.G - w.rb * kPRows > 128 ? 2 : 1;
+      wait(&bars.q_full, q_phase);
+      q_phase ^= 1u;
+      wait(&bars.k_full[it & 1], it >> 1);
+      tc_fence_after();
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) issue_s(t, h, it);
+      commit(&bars.k_empty[it & 1]);
+#pragma unroll 1
+      for (int x = 0; x < n && ok; ++x, ++it) {
+        const bool ahead = x + 1 < n;
+        wait(&bars.v_full[it & 1], it >> 1);
+        if (ahead) wait(&bars.k_full[(it + 1) & 1], (it + 1) >> 1);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+          for (int t = 0; t < tiles; ++t) {
+            wait(&bars.p_full[t][h], t ? p_phase[1] : p_phase[0]);
+            tc_fence_after();
+            issue_o(t, h, it, x > 0 || h > 0);
+            if (ahead) issue_s(t, h, it + 1);
+          }
+        p_phase[0] ^= 1u;
+        if (tiles == 2) p_phase[1] ^= 1u;
+        commit(&bars.v_empty[it & 1]);
+        if (ahead) commit(&bars.k_empty[(it + 1) & 1]);
       }
       u = ue;
       if (u >= w.u1 || !w.next(p)) break;
