@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   constexpr int WPG = NW / NG;           // words of one scale group
   constexpr int PART = part_floats<D, NT>();
   static_assert(PART * 4 <= ring_bytes<D, NG>(), "a part fits the ring");
-  using Work = Kv4Work<ROWS, kTile, THREADS, WARPS>;
+  using Work = Kv4Work<ROWS, kTile, THREADS, WARPS, 0>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[WARPS][kStages];
   __shared__ typename Work::Shared s_work;

@@ -34,7 +34,10 @@ constexpr int kPRows = 256;
 constexpr int kPTile = 128;  // keys per step
 constexpr int kPMinTiles = 4;
 
-using Work = Kv4Work<kPRows, kPTile, kPThreads, 1>;
+// What beginning and ending an item costs, in steps (measured on a prompt of 4096 tokens, whose
+// CTAs have between 2 and 14 items: 291, 247, 220, 201 us with 0, 1, 2, 3).
+constexpr int kPLead = 3;
+using Work = Kv4Work<kPRows, kPTile, kPThreads, 1, kPLead>;
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -128,6 +131,9 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
+__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 // Asynchronous 16-byte copy global -> shared; zeros where `in` is false.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
@@ -143,7 +149,7 @@ struct Bars {
   uint64_t k_empty[2], v_empty[2];  // and read by all products
   uint64_t q_full;                  // the queries of an item
   uint64_t s_full[2][2], p_full[2][2];  // [tile][half]: scores formed; probabilities written
-  uint64_t o_done[2];                   // a half's part of O added
+  uint64_t o_done[2][2];                // [tile][half]: an item's last step added to O
 };
 
 // Whether a scale or a minimum (packed pair) is a NaN or an infinity.
@@ -183,9 +189,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       mbar_init(&bars.v_full[i], 4);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_empty[i], 1);
-      mbar_init(&bars.o_done[i], 1);
       for (int h = 0; h < 2; ++h) {
         mbar_init(&bars.s_full[i][h], 1);
+        mbar_init(&bars.o_done[i][h], 1);
         mbar_init(&bars.p_full[i][h], 4);
       }
     }
@@ -217,7 +223,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     const auto wait = [&](uint64_t* bar, uint32_t phase) { ok = __all_sync(~0u, ok && mbar_wait(bar, phase & 1u)); };
     for (long long u = w.u0; u < w.u1;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
-      const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
+      int first, last;
+      w.part_tiles(u, ue, first, last);
       const int rows = w.req.n * p.G - w.rb * kPRows;  // live rows of the block
       const int grow = w.rb * kPRows + t * 128 + row;  // row of the request
       const int j = (int)((uint32_t)grow / (uint32_t)p.G);
@@ -264,7 +271,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
                 sum2[0] = fma2(sum2[0], pack2(f, f), 0ull);
                 sum2[1] = fma2(sum2[1], pack2(f, f), 0ull);
                 if (tile > first || half) {
-                  wait(&bars.o_done[t], o_phase ^ 1u);
+                  // The other half's product came before the scores that took that half's columns.
+                  if (half && tile + 1 == last) wait(&bars.o_done[t][0], o_phase);
+                  else wait(&bars.s_full[t][half ^ 1], half ? s_phase ^ 1u : s_phase);
                   tc_fence_after();
 #pragma unroll 1
                   for (int k = 0; k < D / 16; ++k) {
@@ -285,10 +294,6 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
               exp32<T>(s + 32, c2, off2, at + 16, sum2);
               tmem_wait_st();
             }
-            // A half's scores say that the product two halves ago is done: before the last half is let
-            // go, the one before it is waited for, so that the wait for the last cannot mistake them.
-            if (half && tile + 1 == last) wait(&bars.o_done[t], o_phase ^ 1u);
-            o_phase ^= 1u;  // this half's product completes phase o_phase ^ 1 of o_done
             tc_fence_before();
             warp_arrive(&bars.p_full[t][half]);
           }
@@ -300,12 +305,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         sum = x + y;
       }
 
-      const bool complete = u == w.item && ue == w.item + w.n_tiles;
+      const bool nothing = first == last;  // the run ended before the item's keys
+      const bool complete = u - w.item <= kPLead && ue == w.item + w.n_tiles;
       const int fc = complete ? 0 : w.first_cta(), lc = complete ? 0 : w.last_cta();
-      const int side = w.item < w.u0 ? 0 : 1;
+      const int side = w.u0 - w.item > kPLead ? 0 : 1;
       const bool more = ue < w.u1 && w.next(p);
+      if (nothing) break;
       if (tile_used) {
-        wait(&bars.o_done[t], o_phase ^ 1u);
+        wait(&bars.o_done[t][0], o_phase);
+        wait(&bars.o_done[t][1], o_phase);
+        o_phase ^= 1u;
         tc_fence_after();
       }
       if (complete) {
@@ -360,35 +369,49 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         if (s_last && tile_used) {
           __threadfence();
           const auto slot = [&](int x) { return p.partial + (int64_t)(2 * x + (x == fc ? 1 : 0)) * slot_floats(D); };
+          // Four parts at a time, so that their loads are in flight together; two are the rule.
           float top = -INFINITY, l = 0.0f;
-          for (int x = fc; x <= lc; ++x) top = fmaxf(top, __ldcg(slot(x) + brow));
+          for (int x0 = fc; x0 <= lc; x0 += 4) {
+            float m[4], z[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float* src = slot(min(x0 + y, lc)) + brow;
+              m[y] = __ldcg(src);
+              z[y] = x0 + y <= lc ? __ldcg(src + kPRows) : 0.0f;
+            }
+            const float to = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+            const float at = to == -INFINITY ? 0.0f : to;
+            l *= kv4_exp2((top - at) * c);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) l = fmaf(z[y], kv4_exp2((m[y] - at) * c), l);
+            top = to;
+          }
           const float to = top == -INFINITY ? 0.0f : top;
-          for (int x = fc; x <= lc; ++x)
-            l += __ldcg(slot(x) + kPRows + brow) * kv4_exp2((__ldcg(slot(x) + brow) - to) * c);
           const float inv = l > 0.0f ? 1.0f / l : l;
           if (live) {
 #pragma unroll 1
-            for (int k = 0; k < D / 64; ++k) {
-              float v[64];
+            for (int k = 0; k < D / 32; ++k) {
+              float v[32];
 #pragma unroll
-              for (int e = 0; e < 64; ++e) v[e] = 0.0f;
+              for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+#pragma unroll 2
               for (int x = fc; x <= lc; ++x) {
                 const float f = kv4_exp2((__ldcg(slot(x) + brow) - to) * c);
-                const float* src = slot(x) + 2 * kPRows + (k * 16 * kPRows + brow) * 4;
+                const float* src = slot(x) + 2 * kPRows + (k * 8 * kPRows + brow) * 4;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 8; ++e) {
                   const float4 o = __ldcg(reinterpret_cast<const float4*>(src + e * kPRows * 4));
                   v[4 * e] += o.x * f, v[4 * e + 1] += o.y * f, v[4 * e + 2] += o.z * f, v[4 * e + 3] += o.w * f;
                 }
               }
 #pragma unroll
-              for (int e = 0; e < 64; e += 8) {
+              for (int e = 0; e < 32; e += 8) {
                 uint4 o;
                 o.x = Elem<T>::from_f2(v[e] * inv, v[e + 1] * inv);
                 o.y = Elem<T>::from_f2(v[e + 2] * inv, v[e + 3] * inv);
                 o.z = Elem<T>::from_f2(v[e + 4] * inv, v[e + 5] * inv);
                 o.w = Elem<T>::from_f2(v[e + 6] * inv, v[e + 7] * inv);
-                *reinterpret_cast<uint4*>(out + k * 64 + e) = o;
+                *reinterpret_cast<uint4*>(out + k * 32 + e) = o;
               }
             }
           }
@@ -410,7 +433,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     uint32_t kc[4 * NW], kp[NG], vq[NG], vc[4 * NW], vp[8 * NG];
     for (long long u = w.u0; u < w.u1 && ok;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
-      const int first = w.tile_lo + (int)(u - w.item), last = first + (int)(ue - u);
+      int first, last;
+      w.part_tiles(u, ue, first, last);
+      if (first == last) break;
       const int* table = p.table + (int64_t)w.r * p.table_stride;
       const int n_rec = (w.req.len + kKv4Rec - 1) / kKv4Rec;
       // This warp's two records of a tile: (nth, off) are the block's place in the table and the
@@ -487,10 +512,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       };
       load_k(first);
       load_v(first);
-      // ---- the item's queries, once the previous item's last scores have been formed
-      if (it > 0) ok = mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
-      constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row; rows copied at a time
-      {
+      // The queries of the request's next row block to L2, a token's heads at a time.
+      if (p.q_h == D && w.rb + 1 < w.blocks) {
+        const int j0 = (int)((uint32_t)((w.rb + 1) * kPRows) / (uint32_t)p.G);
+        const int j1 = min((int)((uint32_t)((w.rb + 2) * kPRows - 1) / (uint32_t)p.G), w.req.n - 1);
+        const uint16_t* q0 = p.q + (p.query_start ? (int64_t)w.req.start * p.q_t : w.r * p.q_r) +
+                             (int64_t)(w.kvh * p.G) * p.q_h;
+        for (int j = j0 + key; j <= j1; j += 128) bulk_prefetch_l2(q0 + j * p.q_t, (uint32_t)(p.G * D * 2));
+      }
+      // The item's queries, once the previous item's last scores have been formed.
+      const auto copy_q = [&]() {
+        constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row; rows copied at a time
+        if (it > 0) ok = ok && mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
         const int ch = key % CH, dj = STEP / p.G, dh = STEP % p.G;
         int row = key / CH, j = (int)((uint32_t)(w.rb * kPRows + row) / (uint32_t)p.G);
         int h = w.rb * kPRows + row - j * p.G;
@@ -505,10 +538,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           h += dh;
           if (h >= p.G) h -= p.G, ++j;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      }
-      fence_proxy_async_smem();
-      warp_arrive(&bars.q_full);
+      };
       for (int tile = first; tile < last && ok; ++tile, ++it) {
         const int stage = it & 1;
         const uint32_t phase = (it >> 1) & 1u;
@@ -539,9 +569,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         }
         fence_proxy_async_smem();
         warp_arrive(&bars.k_full[stage]);
+        if (tile == first) copy_q();
         if (tile + 1 < last) {
           advance();
           load_k(tile + 1);
+        }
+        if (tile == first) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          warp_arrive(&bars.q_full);
         }
         if (it >= 2) ok = ok && mbar_wait(&bars.v_empty[stage], phase ^ 1u);
         // ---- values: rows are dims, a chunk is eight tokens
@@ -588,8 +624,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
   } else {
     // ================================================================ products
     constexpr uint32_t idesc_s = make_idesc_f16(128, 64, kBf16), idesc_o = make_idesc_f16(128, D, kBf16);
-    // Descriptors are one 64-bit base and constant steps (16-byte units).  The whole warp walks the
-    // loop, so that the addresses stay warp-uniform, and one elected lane issues.
+    // The whole warp walks the loop, so that descriptors and addresses stay warp-uniform, and one
+    // elected lane issues: a lane that walks alone takes half as long again for a step.
     const uint64_t base = make_sw128_desc(smem_u32(smem));
     uint32_t it = 0, q_phase = 0, p_phase[2] = {0, 0};
     bool ok = true;
@@ -598,60 +634,64 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       const uint64_t a = base + (uint64_t)(t * (OP >> 4)),
                      b = base + (uint64_t)((2 + (x & 1)) * (OP >> 4) + h * (64 * 128 >> 4));
       const uint32_t d = tmem + t * 128 + h * 64;
-      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = ((k / 4) * 128 * 128 + (k % 4) * 32) >> 4;
-          umma_f16(d, a + off, b + off, idesc_s, k > 0);
-        }
-        umma_commit(&bars.s_full[t][h]);
+      for (int k = 0; k < D / 16; ++k) {
+        const uint64_t off = ((k / 4) * 128 * 128 + (k % 4) * 32) >> 4;
+        umma_f16(d, a + off, b + off, idesc_s, k > 0);
       }
-      __syncwarp();
+      umma_commit(&bars.s_full[t][h]);
     };
     const auto issue_o = [&](int t, int h, uint32_t x, bool accumulate) {
       const uint64_t b = base + (uint64_t)((4 + (x & 1)) * (OP >> 4) + h * (D * 128 >> 4));
       const uint32_t a = tmem + t * 128 + h * 64, d = tmem + 256 + t * 128;
-      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16_ts(d, a + k * 8, b + (k * 32 >> 4), idesc_o, k > 0 || accumulate);
-        umma_commit(&bars.o_done[t]);
-      }
-      __syncwarp();
-    };
-    const auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
+      for (int k = 0; k < 4; ++k) umma_f16_ts(d, a + k * 8, b + (k * 32 >> 4), idesc_o, k > 0 || accumulate);
     };
     for (long long u = w.u0; u < w.u1 && ok;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
-      const int n = (int)(ue - u), tiles = w.req.n * p.G - w.rb * kPRows > 128 ? 2 : 1;
+      int first, last;
+      w.part_tiles(u, ue, first, last);
+      const int n = __shfl_sync(~0u, last - first, 0);
+      const int tiles = __shfl_sync(~0u, w.req.n * p.G - w.rb * kPRows > 128 ? 2 : 1, 0);
+      if (n == 0) break;
+      wait(&bars.k_full[it & 1], it >> 1);
       wait(&bars.q_full, q_phase);
       q_phase ^= 1u;
-      wait(&bars.k_full[it & 1], it >> 1);
       tc_fence_after();
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-        for (int t = 0; t < tiles; ++t) issue_s(t, h, it);
-      commit(&bars.k_empty[it & 1]);
+      if (elect_one()) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (t < tiles) issue_s(t, h, it);
+        umma_commit(&bars.k_empty[it & 1]);
+      }
+      __syncwarp();
 #pragma unroll 1
       for (int x = 0; x < n && ok; ++x, ++it) {
         const bool ahead = x + 1 < n;
         wait(&bars.v_full[it & 1], it >> 1);
         if (ahead) wait(&bars.k_full[(it + 1) & 1], (it + 1) >> 1);
-#pragma unroll 1
+#pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-          for (int t = 0; t < tiles; ++t) {
-            wait(&bars.p_full[t][h], t ? p_phase[1] : p_phase[0]);
-            tc_fence_after();
-            issue_o(t, h, it, x > 0 || h > 0);
-            if (ahead) issue_s(t, h, it + 1);
-          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (t < tiles) {
+              wait(&bars.p_full[t][h], p_phase[t]);
+              tc_fence_after();
+              if (elect_one()) {
+                issue_o(t, h, it, x > 0 || h > 0);
+                if (ahead) issue_s(t, h, it + 1);
+                else umma_commit(&bars.o_done[t][h]);
+                if (h == 1 && t == tiles - 1) {
+                  umma_commit(&bars.v_empty[it & 1]);
+                  if (ahead) umma_commit(&bars.k_empty[(it + 1) & 1]);
+                }
+              }
+              __syncwarp();
+            }
         p_phase[0] ^= 1u;
         if (tiles == 2) p_phase[1] ^= 1u;
-        commit(&bars.v_empty[it & 1]);
-        if (ahead) commit(&bars.k_empty[(it + 1) & 1]);
       }
       u = ue;
       if (u >= w.u1 || !w.next(p)) break;

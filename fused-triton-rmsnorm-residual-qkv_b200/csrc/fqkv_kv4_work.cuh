@@ -43,7 +43,9 @@ __device__ __forceinline__ long long kv4_muldiv(long long x, long long y, long l
 }
 
 // POINTS: 1, or the block's warps; the run of the CTA or of each of its warps starts there.
-template <int ROWS, int TILE, int THREADS, int POINTS>
+// LEAD: an item counts as LEAD tiles more than it reads, in front of them, for what it costs to
+// begin and to end one; a run that starts or ends among them starts or ends with the item.
+template <int ROWS, int TILE, int THREADS, int POINTS, int LEAD>
 struct Kv4Work {
   struct Shared {
     long long scan[THREADS / 32];
@@ -54,8 +56,9 @@ struct Kv4Work {
 
   long long total, u0, u1;  // all tiles, this CTA's run
   long long a, b;           // this warp's part of it (POINTS > 1)
-  // The current item: request r, KV head, row block; its tiles [tile_lo, tile_lo + n_tiles), the
-  // first of which is tile `item` of the batch; row blocks of the request.
+  // The current item: request r, KV head, row block; tiles [item, item + n_tiles) of the batch, of
+  // which the first LEAD stand for nothing and the others for the keys' tiles from tile_lo on; row
+  // blocks of the request.
   long long item;
   Kv4Request req;
   int ctas;   // CTAs that have work
@@ -71,7 +74,13 @@ struct Kv4Work {
     int lo = 0;
     if (p.window > 0) lo = max(0, q.len - q.n + (int)((uint32_t)(rb * ROWS) / (uint32_t)p.G) - p.window + 1);
     tile_lo = lo / TILE;
-    n_tiles = max(1, (hi + TILE - 1) / TILE - tile_lo);
+    n_tiles = max(1, (hi + TILE - 1) / TILE - tile_lo) + LEAD;
+  }
+
+  // The keys' tiles [first, last) of the part [u, ue) of the current item.
+  __device__ __forceinline__ void part_tiles(long long u, long long ue, int& first, int& last) const {
+    first = tile_lo + max(0, (int)(u - item) - LEAD);
+    last = tile_lo + max(0, (int)(ue - item) - LEAD);
   }
 
   static __device__ __forceinline__ int row_blocks(const Kv4AttnParams& p, const Kv4Request& q) {
@@ -253,13 +262,13 @@ struct Kv4Work {
     return true;
   }
 
-  // First and last CTA that have a part of the current item; a CTA's part goes to workspace slot
+  // First and last CTA that have keys of the current item; a CTA's part goes to workspace slot
   // 2 * cta (the item began before its run) or 2 * cta + 1.
   __device__ __forceinline__ int owner(long long tile) const {
     return small ? (int)(((uint32_t)(tile + 1) * (uint32_t)ctas - 1) / (uint32_t)total)
                  : (int)(((tile + 1) * ctas - 1) / total);
   }
-  __device__ __forceinline__ int first_cta() const { return owner(item); }
+  __device__ __forceinline__ int first_cta() const { return owner(item + LEAD); }
   __device__ __forceinline__ int last_cta() const { return owner(item + n_tiles - 1); }
 };
 
