@@ -114,10 +114,10 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
 }
 
 // Warps of a CTA: two CTAs of eight on an SM for eight rows, one of twelve for sixteen rows (170
-// registers a thread); seven where eight rings of the largest records leave no room.
+// registers a thread); fewer where the rings of larger records leave no room.
 template <int D, int NG, int NT>
 constexpr int warps() {
-  return NT == 2 ? (D == 128 && NG == 4 ? 11 : 12) : D == 128 && NG == 4 ? 7 : 8;
+  return NT == 2 ? (D == 128 && NG == 4 ? 10 : D == 128 && NG == 2 ? 11 : 12) : D == 128 ? (NG == 4 ? 6 : NG == 2 ? 7 : 8) : 8;
 }
 template <int D, int NG>
 constexpr int ring_bytes() {
@@ -129,9 +129,15 @@ template <int D, int NT>
 constexpr int part_floats() {
   return 8 * NT * (D + 4);
 }
+// A stage's parameters as the lanes use them, per token and group: the values' {s, r, z, log2 of
+// the token's largest s}, then the keys' {s, m}.
+template <int NG>
+constexpr int param_bytes() {
+  return kTile * NG * 24;
+}
 template <int D, int NG, int NT>
 constexpr int smem_bytes() {
-  return warps<D, NG, NT>() * (ring_bytes<D, NG>() + part_floats<D, NT>() * 4);
+  return warps<D, NG, NT>() * (ring_bytes<D, NG>() + part_floats<D, NT>() * 4 + param_bytes<NG>());
 }
 
 // What the join needs to know of a warp's part of an item.
@@ -162,13 +168,15 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   const int g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * ring_bytes<D, NG>();
   float* parts = reinterpret_cast<float*>(smem + WARPS * ring_bytes<D, NG>());
+  float4* pv = reinterpret_cast<float4*>(smem + WARPS * (ring_bytes<D, NG>() + PART * 4) + warp * param_bytes<NG>());
+  float2* pk = reinterpret_cast<float2*>(pv + kTile * NG);
   // Slot 0: a part that the warp finished before its run ended.  Slot 1: its last part, in the
   // ring, which is idle by then.
   const auto part_at = [&](int w, int slot) -> float* {
     return slot ? reinterpret_cast<float*>(smem + w * ring_bytes<D, NG>()) : parts + w * PART;
   };
   if (tid < WARPS * kStages) {
-    mbar_init(&s_bar[tid / kStages][tid % kStages], 1);
+    mbar_init(&s_bar[tid / kStages][tid % kStages], 2);  // a tile's two records
     fence_mbarrier_init_cluster();
   }
   pdl_wait();
@@ -191,7 +199,7 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   const uint8_t *src = nullptr, *src_next = nullptr;  // records 2 src_tile + lane, and the 32 after them
   int src_tile = 0, ahead_tile, ahead_end;  // next tile to copy, end of this item's part of the run
   int stage_in = 0;
-  long long ahead = w.a;
+  int to_copy = (int)(run_end - w.a);
   const auto address = [&](int rec) {
     const Work& x = s_ahead[warp];
     return kv4_record(p, p.table + (int64_t)x.r * p.table_stride, rec, (x.req.len + kKv4Rec - 1) / kKv4Rec,
@@ -199,14 +207,15 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   };
   const auto enter = [&]() {
     const Work& x = s_ahead[warp];
-    ahead_tile = x.tile_lo + (int)(ahead - x.item);
+    const long long at = run_end - to_copy;
+    ahead_tile = x.tile_lo + (int)(at - x.item);
     ahead_end = x.tile_lo + (int)(min(run_end, x.item + x.n_tiles) - x.item);
     src_tile = ahead_tile;
     src = address(2 * ahead_tile + lane);
     src_next = 2 * ahead_end > 2 * ahead_tile + 32 ? address(2 * ahead_tile + 32 + lane) : nullptr;
   };
   const auto copy_next = [&]() {
-    if (ahead >= run_end) return;
+    if (to_copy <= 0) return;
     if (ahead_tile == ahead_end) {
       Work x = s_ahead[warp];
       __syncwarp();
@@ -220,17 +229,21 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
       src_tile += 16;
       if (ahead_end > src_tile + 16) src_next = address(2 * (src_tile + 16) + lane);
     }
-    const int left = (s_ahead[warp].req.len + kKv4Rec - 1) / kKv4Rec - 2 * ahead_tile;  // records from here on
-    if (lane == 0)
-      mbar_arrive_expect_tx(&s_bar[warp][stage_in], (uint32_t)(left >= 2 ? 2 : max(left, 0)) * REC);
-    __syncwarp();
-    const uint32_t k = (uint32_t)(lane - 2 * (ahead_tile - src_tile));  // 0, 1: the lanes of this tile's records
-    if (k < 2 && src) bulk_load(smem_u32(ring + (stage_in * 2 + k) * REC), src, REC, &s_bar[warp][stage_in]);
-    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    const uint32_t k = (uint32_t)(lane - 2 * (ahead_tile - src_tile));
+    if (k < 2) {  // the lanes of this tile's records; past the last record there is nothing to wait for
+      if (src) {
+        mbar_arrive_expect_tx(&s_bar[warp][stage_in], REC);
+        bulk_load(smem_u32(ring + (stage_in * 2 + k) * REC), src, REC, &s_bar[warp][stage_in]);
+      } else {
+        mbar_arrive(&s_bar[warp][stage_in]);
+      }
+    }
+    stage_in ^= 1;
     ++ahead_tile;
-    ++ahead;
+    --to_copy;
   };
-  if (ahead < run_end) enter();
+  static_assert(kStages == 2, "stages alternate");
+  if (to_copy > 0) enter();
 #pragma unroll
   for (int s = 0; s < kStages; ++s) copy_next();
 
@@ -342,16 +355,47 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
       mbar_wait(&s_bar[warp][stage], (parity >> stage) & 1u);
       parity ^= 1u << stage;
       const uint8_t* rec = ring + stage * 2 * REC;
+      // ---- parameters: each lane prepares one token's
+      {
+        const uint8_t* at = rec + (lane >> 4) * REC + 16 * D + (lane & 15) * NG * 4;
+        uint32_t wk[NG], wv[NG];
+        lds_words<NG>(at, wk);
+        lds_words<NG>(at + 64 * NG, wv);
+        float sv[NG], mv[NG], widest = 0.0f;
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          unpack2<T>(wv[grp], sv[grp], mv[grp]);
+          // A scale of zero goes with codes of zero; any scale then stands for the same numbers.
+          if (sv[grp] == 0.0f) sv[grp] = fmaxf(fabsf(mv[grp]), 1e-20f);
+          widest = fmaxf(widest, sv[grp]);
+        }
+        float lg = log2_approx(widest);
+        if (!(fabsf(lg) < 1e9f)) lg = 0.0f;  // not finite: whoever sees the key becomes NaN
+        __syncwarp();                        // the previous tile's have been read
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          // The offset part p (m + 8 s) is formed from the rounded weight x = p s as x (m / s + 8),
+          // so that both parts of p v carry the same rounding and a value near zero keeps a small
+          // error; where the offset is far larger than the scale, from p itself, so that a weight
+          // too small for fp16 loses nothing of it.
+          const float q = quotient(mv[grp], sv[grp]) + 8.0f;
+          const bool small = fabsf(q) <= 16.0f;
+          float sk, mk;
+          unpack2<T>(wk[grp], sk, mk);
+          pv[lane * NG + grp] =
+              make_float4(sv[grp], small ? q : 0.0f, small ? 0.0f : fmaf(8.0f, sv[grp], mv[grp]), lg);
+          pk[lane * NG + grp] = make_float2(sk, mk);
+        }
+        __syncwarp();
+      }
       // ---- scores, in units of log2: s[record][nt][key g: cols, key g + 8: cols]
       float s[2][NT][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const uint8_t* k = rec + m * REC;
-        uint32_t wa[NW], wb[NW], pa[NG], pb[NG];
+        uint32_t wa[NW], wb[NW];
         lds_words<NW>(k + g * (D / 2) + c * (D / 8), wa);
         lds_words<NW>(k + (g + 8) * (D / 2) + c * (D / 8), wb);
-        lds_words<NG>(k + 16 * D + g * NG * 4, pa);
-        lds_words<NG>(k + 16 * D + (g + 8) * NG * 4, pb);
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
           float acc[NT][4];
@@ -370,15 +414,13 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
               mma16816(acc[nt], a1, qf[nt][i][2], qf[nt][i][3]);
             }
           }
-          float sa, ma, sb, mb;
-          unpack2<T>(pa[grp], sa, ma);
-          unpack2<T>(pb[grp], sb, mb);
+          const float2 ka = pk[(m * kKv4Rec + g) * NG + grp], kb = pk[(m * kKv4Rec + g + 8) * NG + grp];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = (e < 2 ? ma : mb) * qs[nt][grp][e & 1];
-              s[m][nt][e] = fmaf(e < 2 ? sa : sb, acc[nt][e], grp ? s[m][nt][e] + v : v);
+              const float v = (e < 2 ? ka.y : kb.y) * qs[nt][grp][e & 1];
+              s[m][nt][e] = fmaf(e < 2 ? ka.x : kb.x, acc[nt][e], grp ? s[m][nt][e] + v : v);
             }
         }
 #pragma unroll
@@ -399,32 +441,13 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
               if (!seen) s[m][nt][e] = -INFINITY;
             }
       }
-      // ---- the values' parameters.  The reference exponent is that of p s, so that the weights
-      // p s are at most 1 and fp16 holds them whatever the scales.
-      float sv[2][2][NG], mv[2][2][NG], lg[2][2];  // record, key g or g + 8
+      // ---- the reference exponent is that of p s, so that the weights p s are at most 1 and fp16
+      // holds them whatever the scales
+      float lg[2][2];  // record, key g or g + 8
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t pv[NG];
-          lds_words<NG>(rec + m * REC + 16 * D + 64 * NG + (g + 8 * y) * NG * 4, pv);
-          float widest = 0.0f;
-#pragma unroll
-          for (int grp = 0; grp < NG; ++grp) {
-            unpack2<T>(pv[grp], sv[m][y][grp], mv[m][y][grp]);
-            // A scale of zero goes with codes of zero; any scale then stands for the same numbers.
-            if (sv[m][y][grp] == 0.0f) sv[m][y][grp] = fmaxf(fabsf(mv[m][y][grp]), 1e-20f);
-            widest = fmaxf(widest, sv[m][y][grp]);
-          }
-          lg[m][y] = log2_approx(widest);
-        }
-      if (!whole) {  // a key that no row sees may carry anything
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if (!(fabsf(lg[m][y]) < 1e9f)) lg[m][y] = 0.0f;
-      }
+        for (int y = 0; y < 2; ++y) lg[m][y] = pv[(m * kKv4Rec + g + 8 * y) * NG].w;
       // ---- running reference and rescale
       bool grew = false;
       float now[NT][2];
@@ -484,23 +507,13 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
         uint32_t pf[NT][NG][2];
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
-          // The offset part p (m + 8 s) is formed from the rounded weight x = p s as x (m / s + 8),
-          // so that both parts of p v carry the same rounding and a value near zero keeps a small
-          // error; where the offset is far larger than the scale, from p itself, so that a weight
-          // too small for fp16 loses nothing of it.
-          float r[2], z[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float q = quotient(mv[m][y][grp], sv[m][y][grp]) + 8.0f;
-            const bool small = fabsf(q) <= 16.0f;
-            r[y] = small ? q : 0.0f;
-            z[y] = small ? 0.0f : fmaf(8.0f, sv[m][y][grp], mv[m][y][grp]);
-          }
+          const float4 va4 = pv[(m * kKv4Rec + g) * NG + grp], vb4 = pv[(m * kKv4Rec + g + 8) * NG + grp];
+          const float r[2] = {va4.y, vb4.y}, z[2] = {va4.z, vb4.z};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float x[4], b[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = s[m][nt][e] * sv[m][e >> 1][grp];
+            for (int e = 0; e < 4; ++e) x[e] = s[m][nt][e] * (e < 2 ? va4.x : vb4.x);
             if (!whole) {  // a key that is not seen may carry NaN parameters
 #pragma unroll
               for (int e = 0; e < 4; ++e)
