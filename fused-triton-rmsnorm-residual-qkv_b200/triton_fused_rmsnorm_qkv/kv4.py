@@ -26,6 +26,8 @@ from . import _lib
 from .kernel import _DTYPE_CODE, _current_device, _current_stream, _grid_workspace
 
 RECORD_TOKENS = 16
+# Query rows beyond which the library always takes its kernel for prompts (any bound is correct).
+_SPLIT_MAX_ROWS = 1024
 
 
 class KV4Cache:
@@ -102,38 +104,48 @@ def kv4_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_size: int 
     return KV4Cache(data, head_dim=head_dim, block_size=block_size, group_size=group_size, dtype=dtype)
 
 
+_I32 = torch.int32
+
+
 def _int32(name: str, t: torch.Tensor, index: int, numel: Optional[int] = None) -> int:
     """Address of a contiguous int32 vector on device ``index``."""
+    if (t.dtype is _I32 and t.get_device() == index and t.dim() == 1 and t.is_contiguous()
+            and (numel is None or t.numel() == numel)):
+        return t.data_ptr()
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
-    if t.dim() != 1 or (numel is not None and t.shape[0] != numel) or (t.shape[0] > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous vector" + (f" of {numel}" if numel is not None else "")
-                         + f", got shape {tuple(t.shape)}")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous vector" + (f" of {numel}" if numel is not None else "")
+                     + f", got shape {tuple(t.shape)}")
 
 
 def _table(t: torch.Tensor, index: int, rows: int):
     """(address, row stride, width) of block tables (rows, width) with unit column stride."""
-    if t.dtype != torch.int32:
+    if t.dtype is not _I32:
         raise TypeError(f"block_tables must be int32, got {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"block_tables is on {t.device}, expected cuda:{index}")
-    if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"block_tables must be ({rows}, width) with unit column stride, got {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0) if rows > 1 else t.shape[1], t.shape[1]
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == rows:
+        width = shape[1]
+        stride, unit = t.stride()
+        if unit == 1 or width <= 1:
+            return t.data_ptr(), stride if rows > 1 else width, width
+    raise ValueError(f"block_tables must be ({rows}, width) with unit column stride, got {tuple(shape)}")
 
 
 def _run(index: int, name: str, *args) -> None:
     """Call ``fqkv_kv4_<name>`` with device ``index`` current, appending its flags and stream."""
-    if _lib._lib is None:
+    call = _lib.kv4.get(name)
+    if call is None:
         _lib.load()
+        call = _lib.kv4[name]
     if index == _current_device():
-        rc = _lib.kv4[name](*args, _lib.FLAG_PDL, _current_stream(index))
+        rc = call(*args, _lib.FLAG_PDL, _current_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = _lib.kv4[name](*args, _lib.FLAG_PDL, _current_stream(index))
+            rc = call(*args, _lib.FLAG_PDL, _current_stream(index))
     if rc:
         _lib.check(rc, f"fqkv_kv4_{name}")
 
@@ -167,8 +179,7 @@ def kv4_plan(
     the free list cannot serve is refused: no blocks, ``seq_lens`` 0, slots -1.
     """
     assert context_lens.is_cuda, "kv4_plan requires CUDA tensors"
-    index = context_lens.get_device()
-    R = context_lens.shape[0] if context_lens.dim() == 1 else -1
+    index, R = context_lens.get_device(), context_lens.numel()
     ctx, new = _int32("context_lens", context_lens, index), _int32("new_lens", new_lens, index, R)
     table, stride, width = _table(block_tables, index, R)
     free, count = _int32("free_blocks", free_blocks, index), _int32("n_free", n_free, index, 1)
@@ -176,8 +187,8 @@ def kv4_plan(
         raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
     sizes = (R + 1, n_tokens, n_tokens, R, 1, 1)
     if out is None:
-        buf = torch.empty(2 * (R + n_tokens) + 3, dtype=torch.int32, device=context_lens.device)
-        out = KV4Plan(*buf.split(sizes))
+        buf = context_lens.new_empty(2 * (R + n_tokens) + 3)
+        out = KV4Plan._make(buf.split_with_sizes(sizes))
         base, at = buf.data_ptr(), []
         for n in sizes:
             at.append(base)
@@ -191,7 +202,7 @@ def kv4_plan(
 def _kv_rows(name: str, t: torch.Tensor, cache: KV4Cache):
     """(tensor, batch, tokens per batch, strides of batch, token, head) of keys or values given
     as (tokens, n_kv, D) or head-major (B, n_kv, S, D)."""
-    if t.dtype != cache.dtype:
+    if t.dtype is not cache.dtype:
         raise TypeError(f"{name} must be {cache.dtype}, got {t.dtype}")
     if t.get_device() != cache.index:
         raise ValueError(f"{name} is on {t.device}, the cache is on {cache.device}")
@@ -206,9 +217,10 @@ def _kv_rows(name: str, t: torch.Tensor, cache: KV4Cache):
 
 
 def _aligned_rows(t: torch.Tensor):
-    """``t`` and its strides; a contiguous copy where the kernels' 16-byte loads need one."""
+    """``t`` (three or four dims) and its strides; a contiguous copy where the kernels' 16-byte
+    loads need one."""
     st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(s % 8 for s in st[:-1]):
+    if st[-1] != 1 or (st[0] | st[1] | st[-2]) & 7 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         st = t.stride()
     return t, st
@@ -235,14 +247,16 @@ def kv4_gather(cache: KV4Cache, slots: torch.Tensor):
     """What ``slots`` hold, as numbers: ``(k, v)``, each (tokens, n_kv_heads, D) in the cache's
     dtype, zeros for a negative slot."""
     at = _int32("slots", slots, cache.index)
-    n = slots.shape[0]
-    k, v = torch.empty(2, n, cache.n_kv_heads, cache.head_dim, dtype=cache.dtype, device=cache.device).unbind(0)
+    n = slots.numel()
+    k = slots.new_empty((n, cache.n_kv_heads, cache.head_dim), dtype=cache.dtype)
+    v = torch.empty_like(k)
     if n:
         _run(cache.index, "gather", cache._ptr, at, n, k.data_ptr(), v.data_ptr())
     return k, v
 
 
-_workspace: dict = {}  # (n_q, n_kv, D, bound) -> bytes the library asks for
+# (n_q, n_kv, D, queries, at most 1 + the most the split kernel takes) -> bytes the library asks for.
+_workspace: dict = {}
 
 
 def kv4_attention(
@@ -278,7 +292,7 @@ def kv4_attention(
     """
     assert q.is_cuda, "kv4_attention requires CUDA tensors"
     D, index = cache.head_dim, cache.index
-    if q.dtype != cache.dtype:
+    if q.dtype is not cache.dtype:
         raise TypeError(f"q must be {cache.dtype}, got {q.dtype}")
     if q.get_device() != index:
         raise ValueError(f"q is on {q.device}, the cache is on {cache.device}")
@@ -289,7 +303,7 @@ def kv4_attention(
     q, st = _aligned_rows(q)
     n_q = shape[1]
     lens = _int32("seq_lens", seq_lens, index)
-    R = seq_lens.shape[0]
+    R = seq_lens.numel()
     starts = None
     if len(shape) == 4:
         if query_start is not None:
@@ -317,7 +331,7 @@ def kv4_attention(
         raise ValueError(f"window must be positive, got {window}")
     table, stride, width = _table(block_tables, index, R)
     if out is None:
-        out = torch.empty(want, dtype=q.dtype, device=q.device)
+        out = q.new_empty(want)
         o_t = n_q * D
     else:
         if out.shape != want or out.dtype != q.dtype or out.get_device() != index:
@@ -328,7 +342,7 @@ def kv4_attention(
         o_t = rows.stride(0) if T > 1 else n_q * D
     if T == 0 or R == 0:
         return out
-    key = (n_q, cache.n_kv_heads, D, bound)
+    key = (n_q, cache.n_kv_heads, D, min(bound, _SPLIT_MAX_ROWS + 1))
     need = _workspace.get(key)
     if need is None:
         need = _workspace[key] = _lib.load().fqkv_kv4_workspace_bytes(*key)
