@@ -1,7 +1,7 @@
 // fqkv_kv4.cu -- the bookkeeping and storage kernels of the paged 4-bit key/value cache:
 // block tables and slots planned from request lengths, keys and values quantised into their
 // slots, and slots read back as numbers.
-#include "fqkv_kv4.cuh"
+#include "fqkv_kv4_work.cuh"
 
 namespace fqkv {
 namespace {
@@ -130,8 +130,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const Kv4PlanPar
 }
 
 // ---------------------------------------------------------------------------
-// Append and gather: one thread per 8 dims of a token's key or value head; the D / 8 lanes of
-// a head row are neighbours in a warp, so a group's minimum and maximum are shuffles.
+// Append and gather: a thread takes the part of a token's head that is contiguous in the cache,
+// so that codes move in 16-byte pieces (8 at D = 64): for keys the dims 32 i + 8 c .. + 7 of lane
+// c of four, for values 32 i + 4 g .. + 3 of lane g of eight, for all i.  The lanes of a token are
+// neighbours, so a group's minimum and maximum are shuffles.  Bound by the 16-bit numbers' bytes.
 // ---------------------------------------------------------------------------
 constexpr int kStoreThreads = 256;
 
@@ -157,132 +159,203 @@ __device__ __forceinline__ uint8_t* slot_record(const Kv4Cache& c, int slot, int
   return c.data + (((int64_t)block * c.n_kv + head) * (c.P / kKv4Rec) + at / kKv4Rec) * rec_bytes;
 }
 
-// 16-bit word of the values (h, g, c, i, b): token t = 8 h + 2 c + b, dims 32 i + 4 g .. + 3.
+// Byte offset among the values' codes of the NW words (i = 0 .. NW - 1) of token t's pair, lane g.
 template <int D>
-__device__ __forceinline__ int value_word(int t, int i, int g) {
-  const int h = t >> 3, c = (t >> 1) & 3, b = t & 1;
-  return D == 128 ? ((h * 32 + g * 4 + c) * 4 + i) * 2 + b : ((g * 4 + c) * 4 + h * 2 + i) * 2 + b;
+__device__ __forceinline__ int value_words(int t, int g) {
+  const int h = t >> 3, c = (t >> 1) & 3;
+  return D == 128 ? (h * 32 + g * 4 + c) * 16 : (g * 4 + c) * 16 + h * 8;
+}
+
+template <int N>
+__device__ __forceinline__ void store_words(uint8_t* p, const uint32_t* w) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+// Minimum and maximum of packed 16-bit pairs; a NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (Kv4Nib<T>::kFullRange) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (Kv4Nib<T>::kFullRange) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// One token's keys (KIND 0) or values (1) of one head: N = 8 or 4 dims per i, LANES lanes a token.
+template <typename T, int D, int NG, int KIND>
+__device__ __forceinline__ void append_rows(const Kv4AppendParams& p, int head) {
+  constexpr int NW = D / 32, N = KIND ? 4 : 8, LANES = 32 / N, REC = kv4_record_bytes(D, NG), WPG = NW / NG;
+  const int64_t token = (int64_t)blockIdx.x * (kStoreThreads / LANES) + threadIdx.x / LANES;
+  const int part = threadIdx.x % LANES;
+  const bool live = token < p.T;
+  const int slot = live ? p.slots[token] : -1;
+  uint32_t x[NW][N / 2] = {};
+  if (live) {  // the numbers do not wait for the slot
+    const int64_t b = p.S == p.T ? 0 : token / p.S, s = token - b * p.S;
+    const uint16_t* src = KIND ? p.v + b * p.v_b + s * p.v_s + head * p.v_h : p.k + b * p.k_b + s * p.k_s + head * p.k_h;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if constexpr (N == 8) *reinterpret_cast<uint4*>(x[i]) = *reinterpret_cast<const uint4*>(src + 32 * i + 8 * part);
+      else *reinterpret_cast<uint2*>(x[i]) = *reinterpret_cast<const uint2*>(src + 32 * i + 4 * part);
+    }
+  }
+  uint32_t param[NG];
+  float low[NG], scale[NG];
+  bool bad = false;
+#pragma unroll
+  for (int grp = 0; grp < NG; ++grp) {
+    uint32_t lo = x[grp * WPG][0], hi = lo;
+#pragma unroll
+    for (int i = grp * WPG; i < (grp + 1) * WPG; ++i)
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        lo = min2<T>(lo, x[i][e]);
+        hi = max2<T>(hi, x[i][e]);
+      }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+      lo = min2<T>(lo, __shfl_xor_sync(~0u, lo, o));
+      hi = max2<T>(hi, __shfl_xor_sync(~0u, hi, o));
+    }
+    lo = min2<T>(lo, __byte_perm(lo, lo, 0x1032));
+    hi = max2<T>(hi, __byte_perm(hi, hi, 0x1032));
+    // The minimum is one of the 16-bit inputs, so it is stored exactly; the scale is rounded once,
+    // and the codes are formed with the rounded scale that a reader multiplies them by.
+    low[grp] = Elem<T>::to_f((uint16_t)lo);
+    const uint16_t scale16 = Elem<T>::from_f(__fmul_rn(Elem<T>::to_f((uint16_t)hi) - low[grp], 1.0f / 15.0f));
+    scale[grp] = Elem<T>::to_f(scale16);
+    bad |= non_finite<T>((uint16_t)lo) || non_finite<T>((uint16_t)hi) || non_finite<T>(scale16);
+    param[grp] = (uint32_t)scale16 | (lo << 16);
+  }
+  // (the groups' extremes, and so `bad`, are the same in all lanes of the token)
+  // Codes clamp(rint(d / s), 0, 15), d = x - minimum >= 0, with the quotient correctly rounded
+  // first.  d times an approximate reciprocal is off by less than 4e-6, so only a quotient that
+  // close to a half is divided out (16-bit numbers meet halves often enough that a whole thread's
+  // codes are not done again for one).  Adding 1.5 * 2^23 rounds and leaves the code in the low
+  // bits.  N codes per word: pairs of dims (2 j, 2 j + 1) at bits (4 j, 16 + 4 j) for keys, dim j
+  // at bits 4 j for values.
+  uint32_t w[NW];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const float s = scale[i / WPG], lo = low[i / WPG];
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    // (nothing passes where the reciprocal is not normal)
+    const float tight = s > 1e-37f && s < 1e37f ? 0.49999f : -1.0f;
+    w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = Elem<T>::to_f((uint16_t)(e & 1 ? x[i][e / 2] >> 16 : x[i][e / 2])) - lo;
+      const float q = fminf(d * inv, 15.0f);
+      float r = __fadd_rn(q, 12582912.0f);
+      if (!(fabsf(q - __fadd_rn(r, -12582912.0f)) < tight)) r = __fadd_rn(fminf(__fdiv_rn(d, s), 15.0f), 12582912.0f);
+      w[i] |= (__float_as_uint(r) & 15u) << (KIND ? 4 * e : 4 * (e >> 1) + 16 * (e & 1));
+    }
+    if (!(s > 0.0f)) w[i] = 0;
+  }
+  if (bad) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) w[i] = 0;
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) param[grp] = 0x7FFF7FFFu;  // NaN in both types
+  }
+  uint8_t* rec = slot_record(p.c, slot, head, REC);
+  const int t = slot & (kKv4Rec - 1);
+  if constexpr (KIND == 0) {
+    if (rec) store_words<NW>(rec + t * (D / 2) + part * (D / 8), w);
+  } else {
+    // Tokens 2 c and 2 c + 1 share 32-bit words.  When the token before or after this one in the
+    // call is the other of the pair and in this warp, each of the two writes half of the words.
+    const int from = ((int)(threadIdx.x & 31) + (t & 1 ? -LANES : LANES)) & 31;
+    const bool near = t & 1 ? (int)(threadIdx.x & 31) >= LANES : (int)(threadIdx.x & 31) < 32 - LANES;
+    const int other_slot = __shfl_sync(~0u, slot, from);
+    uint32_t o[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) o[i] = __shfl_sync(~0u, w[i], from);
+    // The other token pairs with this one only if it chose this lane as its partner too.
+    if (rec) {
+      uint8_t* at = rec + 8 * D + value_words<D>(t, part);
+      if (near && slot >= 0 && other_slot == (slot ^ 1)) {
+        uint32_t both[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) both[i] = t & 1 ? o[i] | (w[i] << 16) : w[i] | (o[i] << 16);
+        if (t & 1) store_words<NW / 2>(at + 2 * NW, both + NW / 2);
+        else store_words<NW / 2>(at, both);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) *reinterpret_cast<uint16_t*>(at + 4 * i + 2 * (t & 1)) = (uint16_t)w[i];
+      }
+    }
+  }
+  if (rec && part == 0) store_words<NG>(rec + 16 * D + KIND * 64 * NG + t * NG * 4, param);
 }
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kStoreThreads) kv4_append_kernel(const Kv4AppendParams p) {
-  constexpr int LPR = D / 8, LPG = LPR / NG, REC = kv4_record_bytes(D, NG);
   pdl_wait();
   pdl_launch_dependents();
-  const int kind = (int)blockIdx.y / p.c.n_kv, head = (int)blockIdx.y % p.c.n_kv;
-  const int64_t token = (int64_t)blockIdx.x * (kStoreThreads / LPR) + threadIdx.x / LPR;
-  const int seg = threadIdx.x % LPR;
-  const bool live = token < p.T;
-  const int slot = live ? p.slots[token] : -1;
-  uint16_t x[8] = {};
-  if (slot >= 0) {
-    const int64_t b = token / p.S, s = token - b * p.S;
-    const uint16_t* src = kind == 0 ? p.k + b * p.k_b + s * p.k_s + head * p.k_h
-                                    : p.v + b * p.v_b + s * p.v_s + head * p.v_h;
-    *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src + seg * 8);
-  }
-  float f[8], lo, hi;
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    f[e] = Elem<T>::to_f(x[e]);
-    bad |= non_finite<T>(x[e]);
-    lo = e ? fminf(lo, f[e]) : f[e];
-    hi = e ? fmaxf(hi, f[e]) : f[e];
-  }
-#pragma unroll
-  for (int o = 1; o < LPG; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-  }
-  // The minimum is one of the 16-bit inputs, so it is stored exactly; the scale is rounded once,
-  // and the codes are formed with the rounded scale that a reader multiplies them by.
-  const uint16_t scale16 = Elem<T>::from_f(__fmul_rn(hi - lo, 1.0f / 15.0f));
-  const float scale = Elem<T>::to_f(scale16);
-  bad |= non_finite<T>(scale16);
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) bad |= __shfl_xor_sync(~0u, (int)bad, o) != 0;
-  uint32_t code[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = rintf(__fdiv_rn(f[e] - lo, scale));
-    code[e] = scale > 0.0f && !bad ? (uint32_t)fminf(fmaxf(v, 0.0f), 15.0f) : 0u;
-  }
-  const uint32_t param = bad ? 0x7FFF7FFFu  // NaN in both types
-                             : (uint32_t)scale16 | ((uint32_t)Elem<T>::from_f(lo) << 16);
-  uint8_t* rec = slot_record(p.c, slot, head, REC);
-  const int t = slot & (kKv4Rec - 1);
-  if (kind == 0) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w |= (code[2 * j] << (4 * j)) | (code[2 * j + 1] << (16 + 4 * j));
-    if (rec) {
-      const int i = seg >> 2, c = seg & 3;
-      *reinterpret_cast<uint32_t*>(rec + t * (D / 2) + c * (D / 8) + i * 4) = w;
+  const int head = (int)blockIdx.y >> 1;
+  if (blockIdx.y & 1) append_rows<T, D, NG, 1>(p, head);
+  else if ((int64_t)blockIdx.x * (kStoreThreads / 4) < p.T) append_rows<T, D, NG, 0>(p, head);
+}
+
+template <typename T, int D, int NG, int KIND>
+__device__ __forceinline__ void gather_rows(const Kv4GatherParams& p, int head) {
+  constexpr int NW = D / 32, N = KIND ? 4 : 8, LANES = 32 / N, REC = kv4_record_bytes(D, NG), WPG = NW / NG;
+  const int64_t token = (int64_t)blockIdx.x * (kStoreThreads / LANES) + threadIdx.x / LANES;
+  const int part = threadIdx.x % LANES;
+  if (token >= p.T) return;
+  const int slot = p.slots[token];
+  const uint8_t* rec = slot_record(p.c, slot, head, REC);
+  uint32_t w[NW] = {}, param[NG] = {};
+  if (rec) {
+    const int t = slot & (kKv4Rec - 1);
+    const uint8_t* at = KIND ? rec + 8 * D + value_words<D>(t, part) : rec + t * (D / 2) + part * (D / 8);
+    if constexpr (NW == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(at);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(at);
+      w[0] = v.x, w[1] = v.y;
     }
-  } else {
-    uint32_t half[2] = {0, 0};
+    if constexpr (KIND == 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      half[0] |= code[j] << (4 * j);
-      half[1] |= code[4 + j] << (4 * j);
+      for (int i = 0; i < NW; ++i) w[i] = t & 1 ? w[i] >> 16 : w[i];
     }
-    // Tokens 2 c and 2 c + 1 share 32-bit words.  When the next (previous) row of the warp is
-    // the other token of the pair, each of the two lanes writes one whole word.
-    const int other_slot = __shfl_xor_sync(~0u, slot, LPR);
-    const uint32_t o0 = __shfl_xor_sync(~0u, half[0], LPR), o1 = __shfl_xor_sync(~0u, half[1], LPR);
-    if (rec) {
-      uint16_t* words = reinterpret_cast<uint16_t*>(rec + 8 * D);
-      const int i = seg >> 2, g = 2 * (seg & 3);
-      if (other_slot == (slot ^ 1)) {
-        if (t & 1)
-          *reinterpret_cast<uint32_t*>(words + value_word<D>(t ^ 1, i, g + 1)) = o1 | (half[1] << 16);
-        else
-          *reinterpret_cast<uint32_t*>(words + value_word<D>(t, i, g)) = half[0] | (o0 << 16);
-      } else {
-        words[value_word<D>(t, i, g)] = (uint16_t)half[0];
-        words[value_word<D>(t, i, g + 1)] = (uint16_t)half[1];
-      }
-    }
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(rec + 16 * D + KIND * 64 * NG) + t * NG;
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) param[grp] = q[grp];
   }
-  if (rec && seg % LPG == 0)
-    *reinterpret_cast<uint32_t*>(rec + 16 * D + kind * 64 * NG + (t * NG + seg / LPG) * 4) = param;
+  uint16_t* dst = (KIND ? p.v : p.k) + (token * p.c.n_kv + head) * D + N * part;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const float scale = Elem<T>::to_f((uint16_t)param[i / WPG]), low = Elem<T>::to_f((uint16_t)(param[i / WPG] >> 16));
+    uint32_t o[N / 2];
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      const uint32_t a = KIND ? (w[i] >> (8 * e)) & 15u : (w[i] >> (4 * e)) & 15u;
+      const uint32_t b = KIND ? (w[i] >> (8 * e + 4)) & 15u : (w[i] >> (4 * e + 16)) & 15u;
+      o[e] = Elem<T>::from_f2(__fmaf_rn((float)a, scale, low), __fmaf_rn((float)b, scale, low));
+    }
+    store_words<N / 2>(reinterpret_cast<uint8_t*>(dst + 32 * i), o);
+  }
 }
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kStoreThreads) kv4_gather_kernel(const Kv4GatherParams p) {
-  constexpr int LPR = D / 8, LPG = LPR / NG, REC = kv4_record_bytes(D, NG);
   pdl_wait();
   pdl_launch_dependents();
-  const int kind = (int)blockIdx.y / p.c.n_kv, head = (int)blockIdx.y % p.c.n_kv;
-  const int64_t token = (int64_t)blockIdx.x * (kStoreThreads / LPR) + threadIdx.x / LPR;
-  const int seg = threadIdx.x % LPR;
-  if (token >= p.T) return;
-  const int slot = p.slots[token];
-  const uint8_t* rec = slot_record(p.c, slot, head, REC);
-  uint32_t o[4] = {0, 0, 0, 0};
-  if (rec) {
-    const int t = slot & (kKv4Rec - 1), i = seg >> 2, c = seg & 3;
-    const uint32_t param =
-        *reinterpret_cast<const uint32_t*>(rec + 16 * D + kind * 64 * NG + (t * NG + seg / LPG) * 4);
-    const float scale = Elem<T>::to_f((uint16_t)param), low = Elem<T>::to_f((uint16_t)(param >> 16));
-    uint32_t code[8];
-    if (kind == 0) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + t * (D / 2) + c * (D / 8) + i * 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) code[e] = (w >> (4 * (e >> 1) + 16 * (e & 1))) & 15u;
-    } else {
-      const uint16_t* words = reinterpret_cast<const uint16_t*>(rec + 8 * D);
-      const uint32_t a = words[value_word<D>(t, i, 2 * c)], b = words[value_word<D>(t, i, 2 * c + 1)];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) code[e] = ((e < 4 ? a : b) >> (4 * (e & 3))) & 15u;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      o[e] = Elem<T>::from_f2(__fmaf_rn((float)code[2 * e], scale, low), __fmaf_rn((float)code[2 * e + 1], scale, low));
-  }
-  uint16_t* dst = (kind == 0 ? p.k : p.v) + (token * p.c.n_kv + head) * D + seg * 8;
-  *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  const int head = (int)blockIdx.y >> 1;
+  if (blockIdx.y & 1) gather_rows<T, D, NG, 1>(p, head);
+  else if ((int64_t)blockIdx.x * (kStoreThreads / 4) < p.T) gather_rows<T, D, NG, 0>(p, head);
 }
 
 template <typename F>
@@ -306,7 +379,7 @@ struct AppendLaunch {
   cudaStream_t stream;
   template <typename T, int D, int NG>
   cudaError_t operator()() const {
-    const dim3 grid((unsigned)((p.T * (D / 8) + kStoreThreads - 1) / kStoreThreads), (unsigned)(2 * p.c.n_kv));
+    const dim3 grid((unsigned)((p.T + kStoreThreads / 8 - 1) / (kStoreThreads / 8)), (unsigned)(2 * p.c.n_kv));
     return kv4_launch(kv4_append_kernel<T, D, NG>, grid, kStoreThreads, 0, pdl, stream, p);
   }
 };
@@ -317,7 +390,7 @@ struct GatherLaunch {
   cudaStream_t stream;
   template <typename T, int D, int NG>
   cudaError_t operator()() const {
-    const dim3 grid((unsigned)((p.T * (D / 8) + kStoreThreads - 1) / kStoreThreads), (unsigned)(2 * p.c.n_kv));
+    const dim3 grid((unsigned)((p.T + kStoreThreads / 8 - 1) / (kStoreThreads / 8)), (unsigned)(2 * p.c.n_kv));
     return kv4_launch(kv4_gather_kernel<T, D, NG>, grid, kStoreThreads, 0, pdl, stream, p);
   }
 };
