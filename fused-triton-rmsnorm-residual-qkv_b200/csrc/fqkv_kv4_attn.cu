@@ -58,13 +58,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 // Eight codes of a word as four fp16 pairs (nibbles j and j + 4): 1024 + code for j = 0, 2, where
 // the four bits are the mantissa's lowest, 64 + code for j = 1, 3, where they are bits 4-7.
-__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t& p0, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t low, uint32_t high, uint32_t& p0, uint32_t& p1,
+                                           uint32_t& p2, uint32_t& p3) {
   const uint32_t v = w >> 8;
-  p0 = (w & 0x000F000Fu) | 0x64006400u;
-  p1 = (w & 0x00F000F0u) | 0x54005400u;
-  p2 = (v & 0x000F000Fu) | 0x64006400u;
-  p3 = (v & 0x00F000F0u) | 0x54005400u;
+  p0 = kv4_place<0x000F000Fu>(w, low);
+  p1 = kv4_place<0x00F000F0u>(w, high);
+  p2 = kv4_place<0x000F000Fu>(v, low);
+  p3 = kv4_place<0x00F000F0u>(v, high);
 }
+constexpr uint32_t kMagicLow = 0x64006400u;    // 1024
+constexpr uint32_t kMagicHigh = 0x54005400u;   // 64
 constexpr uint32_t kCentreLow = 0x64086408u;   // 1032 = 1024 + 8
 constexpr uint32_t kCentreHigh = 0x54805480u;  // 72 = 64 + 8
 
@@ -166,6 +169,7 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   __shared__ int s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
+  const uint32_t magic_low = kv4_opaque(kMagicLow, p.n_q), magic_high = kv4_opaque(kMagicHigh, p.n_q);
   uint8_t* ring = smem + warp * ring_bytes<D, NG>();
   float* parts = reinterpret_cast<float*>(smem + WARPS * ring_bytes<D, NG>());
   float4* pv = reinterpret_cast<float4*>(smem + WARPS * (ring_bytes<D, NG>() + PART * 4) + warp * param_bytes<NG>());
@@ -406,8 +410,8 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
 #pragma unroll
           for (int i = grp * WPG; i < (grp + 1) * WPG; ++i) {
             uint32_t a0[4], a1[4];
-            code_pairs(wa[i], a0[0], a0[2], a1[0], a1[2]);
-            code_pairs(wb[i], a0[1], a0[3], a1[1], a1[3]);
+            code_pairs(wa[i], magic_low, magic_high, a0[0], a0[2], a1[0], a1[2]);
+            code_pairs(wb[i], magic_low, magic_high, a0[1], a0[3], a1[1], a1[3]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma16816(acc[nt], a0, qf[nt][i][0], qf[nt][i][1]);
@@ -539,8 +543,8 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
           uint32_t a0[4], a1[4];
-          code_pairs(va[i], a0[0], a0[1], a1[0], a1[1]);
-          code_pairs(vb[i], a0[2], a0[3], a1[2], a1[3]);
+          code_pairs(va[i], magic_low, magic_high, a0[0], a0[1], a1[0], a1[1]);
+          code_pairs(vb[i], magic_low, magic_high, a0[2], a0[3], a1[2], a1[3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             a0[e] = sub_f16x2(a0[e], e & 1 ? kCentreHigh : kCentreLow);

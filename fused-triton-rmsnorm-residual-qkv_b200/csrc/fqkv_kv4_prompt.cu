@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     const int vr = (lane >> 1) & 1, vh = lane & 1, vg = lane >> 2;  // values: record, token half, dim group
     const int rpb = p.c.P / kKv4Rec;
     const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale negates the keys
+    const uint32_t magic = kv4_opaque(Kv4Nib<T>::kOffset2, p.n_q);
     uint32_t it = 0;
     bool ok = true;
     uint32_t kc[4 * NW], kp[NG], vq[NG], vc[4 * NW], vp[8 * NG];
@@ -559,10 +560,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
             const uint32_t x = kc[cc * NW + i];  // dims 32 i + 8 cc ..
             using N = Kv4Nib<T>;
             uint4 v;
-            v.x = N::fma2(N::sub2(N::template pair<0>(x), N::kOffset2), s2, m2);
-            v.y = N::fma2(N::sub2(N::template pair<1>(x), N::kOffset2), s2, m2);
-            v.z = N::fma2(N::sub2(N::template pair<2>(x), N::kOffset2), s2, m2);
-            v.w = N::fma2(N::sub2(N::template pair<3>(x), N::kOffset2), s2, m2);
+            v.x = N::fma2(N::sub2(N::template pair<0>(x, magic), magic), s2, m2);
+            v.y = N::fma2(N::sub2(N::template pair<1>(x, magic), magic), s2, m2);
+            v.z = N::fma2(N::sub2(N::template pair<2>(x, magic), magic), s2, m2);
+            v.w = N::fma2(N::sub2(N::template pair<3>(x, magic), magic), s2, m2);
             const int chunk = 4 * i + cc;
             *reinterpret_cast<uint4*>(k_tile + (chunk / 8) * 128 * 128 + sw128_offset(key, chunk % 8)) = v;
           }
@@ -600,10 +601,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc) {
               const uint32_t x = vc[cc * NW + i];
-              o[0][cc] = N::fma2(N::sub2(N::template pair<0>(x), N::kOffset2), s2[cc], m2[cc]);
-              o[1][cc] = N::fma2(N::sub2(N::template pair<1>(x), N::kOffset2), s2[cc], m2[cc]);
-              o[2][cc] = N::fma2(N::sub2(N::template pair<2>(x), N::kOffset2), s2[cc], m2[cc]);
-              o[3][cc] = N::fma2(N::sub2(N::template pair<3>(x), N::kOffset2), s2[cc], m2[cc]);
+              o[0][cc] = N::fma2(N::sub2(N::template pair<0>(x, magic), magic), s2[cc], m2[cc]);
+              o[1][cc] = N::fma2(N::sub2(N::template pair<1>(x, magic), magic), s2[cc], m2[cc]);
+              o[2][cc] = N::fma2(N::sub2(N::template pair<2>(x, magic), magic), s2[cc], m2[cc]);
+              o[3][cc] = N::fma2(N::sub2(N::template pair<3>(x, magic), magic), s2[cc], m2[cc]);
             }
             const int chunk = (2 * dw + vr) * 2 + vh;  // of 16 chunks of eight keys
 #pragma unroll

@@ -285,8 +285,22 @@ __device__ __forceinline__ const uint8_t* kv4_record(const Kv4AttnParams& p, con
   return p.c.data + (((int64_t)block * p.c.n_kv + kvh) * rpb + (rec - nth * rpb)) * rec_bytes;
 }
 
+// (x & MASK) | magic in one instruction.  `magic` is a register whose value the compiler cannot
+// see (kv4_opaque): two immediates would make it two instructions, and this is the kernels' most
+// frequent one.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t kv4_place(uint32_t x, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(MASK), "r"(magic));
+  return r;
+}
+// `value`, from a number that is never negative.
+__device__ __forceinline__ uint32_t kv4_opaque(uint32_t value, int not_negative) {
+  return value ^ ((uint32_t)not_negative >> 31);
+}
+
 // Four-bit codes as 16-bit floats: nibbles j and j + 4 of w (bits 4 j and 16 + 4 j) as the pair
-// kOffset + code, by placing the four bits in the mantissa of a constant.
+// kOffset + code, by placing the four bits in the mantissa of a constant (kOffset2, opaque).
 template <typename T>
 struct Kv4Nib;
 template <>
@@ -296,8 +310,8 @@ struct Kv4Nib<__nv_bfloat16> {
   static constexpr uint32_t kCentre2 = 0x43084308u;  // 136 = offset + 8
   static constexpr bool kFullRange = true;  // of fp32
   template <int j>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    return ((w >> (4 * j)) & 0x000F000Fu) | kOffset2;
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t magic) {
+    return kv4_place<0x000F000Fu>(w >> (4 * j), magic);
   }
   static __device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t y) {
     uint32_t r;
@@ -317,9 +331,8 @@ struct Kv4Nib<__half> {
   static constexpr uint32_t kCentre2 = 0x54805480u;  // 72 = offset + 8
   static constexpr bool kFullRange = false;
   template <int j>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    const uint32_t x = j == 0 ? w << 4 : w >> (4 * (j > 0 ? j - 1 : 0));
-    return (x & 0x00F000F0u) | kOffset2;
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t magic) {
+    return kv4_place<0x00F000F0u>(j == 0 ? w << 4 : w >> (4 * (j > 0 ? j - 1 : 0)), magic);
   }
   static __device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t y) {
     uint32_t r;
