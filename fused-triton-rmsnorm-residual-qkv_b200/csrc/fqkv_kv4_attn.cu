@@ -33,7 +33,6 @@ namespace fqkv {
 namespace {
 
 constexpr int kTile = 32;    // tokens per ring stage (two records)
-constexpr int kStages = 2;
 
 // Untiled bulk copy global -> shared, counted on a local mbarrier.  Addresses and size are
 // multiples of 16 bytes.
@@ -122,9 +121,14 @@ template <int D, int NG, int NT>
 constexpr int warps() {
   return NT == 2 ? (D == 128 && NG == 4 ? 10 : D == 128 && NG == 2 ? 11 : 12) : D == 128 ? (NG == 4 ? 6 : NG == 2 ? 7 : 8) : 8;
 }
+// Ring stages of a warp, about 9 KB.
+template <int D>
+constexpr int stages() {
+  return D == 128 ? 2 : 4;
+}
 template <int D, int NG>
 constexpr int ring_bytes() {
-  return kStages * 2 * kv4_record_bytes(D, NG);
+  return stages<D>() * 2 * kv4_record_bytes(D, NG);
 }
 // A warp's part of an item as floats: its outputs by column, padded by four floats so that the
 // float4 stores of a quarter-warp (four columns, two dim groups) meet eight different bank groups.
@@ -154,7 +158,7 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
     kv4_attn_split_kernel(const Kv4AttnParams p) {
   constexpr int WARPS = warps<D, NG, NT>(), THREADS = WARPS * 32;
   constexpr int ROWS = 8 * NT;           // query rows of an item
-  constexpr int REC = kv4_record_bytes(D, NG);
+  constexpr int REC = kv4_record_bytes(D, NG), kStages = stages<D>();
   constexpr int NW = D / 32;             // 32-dim blocks: words per lane and key row
   constexpr int WPG = NW / NG;           // words of one scale group
   constexpr int PART = part_floats<D, NT>();
@@ -242,11 +246,10 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
         mbar_arrive(&s_bar[warp][stage_in]);
       }
     }
-    stage_in ^= 1;
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
     ++ahead_tile;
     --to_copy;
   };
-  static_assert(kStages == 2, "stages alternate");
   if (to_copy > 0) enter();
 #pragma unroll
   for (int s = 0; s < kStages; ++s) copy_next();
@@ -634,19 +637,14 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
     o.y = Elem<T>::from_f2(v.z * inv, v.w * inv);
     *reinterpret_cast<uint2*>(p.out + (int64_t)(x.start + j) * p.o_t + (int64_t)(x.head0 + h) * D + dim) = o;
   };
-  int shared_at[2] = {-1, -1};  // entries (warp * 2 + slot) of the items shared with other CTAs
-  for (int x = 0; x < 2 * WARPS;) {
+  // Lane e looks after entry e = warp * 2 + slot; the entries of one item are one ballot.
+  const long long entry = lane < 2 * WARPS ? s_info[lane >> 1][lane & 1].item : -1;
+  int shared_at[2] = {-1, -1};  // an entry of each item shared with other CTAs
+  for (uint32_t left = __ballot_sync(~0u, entry >= 0); left;) {
+    const int x = __ffs(left) - 1;
+    const uint32_t mine = __ballot_sync(~0u, entry == __shfl_sync(~0u, entry, x)) & left;
+    left &= ~mine;
     const PartInfo& info = s_info[x >> 1][x & 1];
-    if (info.item < 0) {
-      ++x;
-      continue;
-    }
-    int y = x + 1, end = y;  // entries [x, end) belong to the item
-    for (; y < 2 * WARPS; ++y) {
-      const long long it = s_info[y >> 1][y & 1].item;
-      if (it >= 0 && it != info.item) break;
-      if (it >= 0) end = y + 1;
-    }
     const bool here = info.item >= any.u0 && info.item + info.n_tiles <= any.u1;
     const int side = info.item < any.u0 ? 0 : 1;
     if (!here) shared_at[side] = x;
@@ -654,15 +652,17 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
     for (int k = tid; k < ROWS * D / 4; k += THREADS) {
       const int col = k / (D / 4), dim = k % (D / 4) * 4;
       float m = -INFINITY, l = 0.0f;
-      for (int z = x; z < end; ++z)
-        if (s_info[z >> 1][z & 1].item >= 0) m = fmaxf(m, s_max[z >> 1][z & 1][col]);
+      for (uint32_t z = mine; z; z &= z - 1) {
+        const int e = __ffs(z) - 1;
+        m = fmaxf(m, s_max[e >> 1][e & 1][col]);
+      }
       const float to = m == -INFINITY ? 0.0f : m;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int z = x; z < end; ++z) {
-        if (s_info[z >> 1][z & 1].item < 0) continue;
-        const float f = kv4_exp2(s_max[z >> 1][z & 1][col] - to);
-        const float4 o = *reinterpret_cast<const float4*>(part_at(z >> 1, z & 1) + col * (D + 4) + dim);
-        l = fmaf(s_sum[z >> 1][z & 1][col], f, l);
+      for (uint32_t z = mine; z; z &= z - 1) {
+        const int e = __ffs(z) - 1;
+        const float f = kv4_exp2(s_max[e >> 1][e & 1][col] - to);
+        const float4 o = *reinterpret_cast<const float4*>(part_at(e >> 1, e & 1) + col * (D + 4) + dim);
+        l = fmaf(s_sum[e >> 1][e & 1][col], f, l);
         v.x = fmaf(o.x, f, v.x), v.y = fmaf(o.y, f, v.y), v.z = fmaf(o.z, f, v.z), v.w = fmaf(o.w, f, v.w);
       }
       if (here) {
@@ -675,7 +675,6 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
         *reinterpret_cast<float4*>(part + 2 * ROWS + col * D + dim) = v;
       }
     }
-    x = y;
   }
   if (shared_at[0] < 0 && shared_at[1] < 0) return;
 
