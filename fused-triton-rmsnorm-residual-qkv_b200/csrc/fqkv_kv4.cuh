@@ -74,10 +74,8 @@ struct Kv4AttnParams {
 cudaError_t launch_kv4_plan(const Kv4PlanParams& p, bool pdl, cudaStream_t stream);
 cudaError_t launch_kv4_append(const Kv4AppendParams& p, bool bf16, bool pdl, cudaStream_t stream);
 cudaError_t launch_kv4_gather(const Kv4GatherParams& p, bool bf16, bool pdl, cudaStream_t stream);
-// Rows per item (8 or 16) by the row count hint.
-cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int row_blocks8, int sms, bool bf16, bool pdl,
-                                  cudaStream_t stream);
-
+cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int sms, bool bf16, bool pdl, cudaStream_t stream);
+int64_t kv4_split_partial_bytes(int D);
 cudaError_t launch_kv4_attn_prompt(const Kv4AttnParams& p, int sms, bool bf16, bool pdl, cudaStream_t stream);
 int64_t kv4_prompt_partial_bytes(int D);
 

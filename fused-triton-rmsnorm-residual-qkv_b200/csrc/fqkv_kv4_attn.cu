@@ -4,13 +4,14 @@
 // Mathematics.  A code c stands for s c + m, with s and m per token and group of dims, so
 //   q . k_t = sum_groups ( s_tg * (q_g . c_tg) + m_tg * sum(q_g) )
 //   sum_t p_t v_t = sum_t (p_t s_tg) (c_tg - 8) + sum_t p_t (m_tg + 8 s_tg).
-// The tensor cores multiply the small integers, exact in 16 bits, and the parameters meet the
-// scores and the probabilities in fp32: no dequantised tile is ever formed.  An integer becomes
-// a 16-bit float by placing its four bits in the mantissa of a constant (128 + c in bf16,
-// 64 + c in fp16): one shift and one three-input logic operation per two codes.  For the keys
-// the constant is taken back by starting the accumulator at -constant * sum(q_g); for the values
-// it is subtracted, and the codes centred, with one packed subtraction, so that the sum over a
-// long context does not cancel a large offset.  p s is rounded to 16 bits for the product (the
+// The tensor cores multiply the small integers, exact in fp16, and the parameters meet the scores
+// and the probabilities in fp32: no dequantised tile is ever formed.  Four bits become an fp16
+// number by placing them in the mantissa of a constant (1024 + c or 64 + c): a word's eight codes
+// cost one shift and four three-input logic operations.  For the keys the constants are taken back
+// by the value the accumulator starts with; for the values they are subtracted and the codes
+// centred, so that the sum over a long context does not cancel a large offset.  bf16 queries are
+// divided by a power of two per row and the weights p s are held at 1 or less by the reference
+// exponent, so fp16 loses nothing of either range.  p s is rounded to 16 bits for the product (the
 // one rounding to fewer than 32 bits besides the output); maxima, sums and outputs are fp32.
 //
 // Shape.  Both products are transposed (keys x queries and dims x queries, m16n8k16), so the
@@ -18,15 +19,18 @@
 // A record's bytes are stored in fragment order: a warp's 16-byte shared loads are conflict
 // free and need no transposition (the values' tokens are interleaved in pairs).
 //
-// Bound: the codes' bytes over HBM.  Per 16 tokens and KV head that is 2176 bytes at D = 128
-// (one group), about 90 cycles of an SM's share of the bandwidth, against about 50 cycles of
-// issue slots for the unpacking, the products and the softmax.
+// Bound: the codes' bytes over HBM, 2176 per 16 tokens and KV head at D = 128 with one group, about
+// 90 cycles of an SM's share of the bandwidth.  Measured (B200, bf16, 64 requests of 1 to 8000
+// tokens, 32 / 8 heads, 288 MB): 85 us, 3.4 TB/s; copies alone 58 us, everything but the products
+// and their unpacking 64 us.  The rest is issue: about 350 instructions a record, of which the
+// logic pipe (one per two cycles and scheduler) takes about half.
 //
 // Split.  The items (request, KV head, block of query rows) are laid end to end as tiles of 32
-// tokens and cut into equal runs, one per CTA, whatever the lengths; inside a CTA each warp
-// takes a contiguous part of a piece with a ring of its own, filled by bulk copies of whole
-// records.  An item cut between CTAs is joined by the CTA that arrives last, which adds the
-// parts in the order of the CTAs, so the result does not depend on the arrival order.
+// tokens and cut into equal runs, one per CTA and within it one per warp, whatever the lengths.  A
+// warp streams its run through a ring of its own, filled by bulk copies of whole records, without
+// a barrier between items; a CTA's warps join their parts once, at the end.  An item cut between
+// CTAs is joined by the CTA that arrives last, which adds the parts in the order of the CTAs, so
+// the result does not depend on the arrival order.
 #include "fqkv_kv4_work.cuh"
 
 namespace fqkv {
@@ -115,11 +119,14 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// Warps of a CTA: two CTAs of eight on an SM for eight rows, one of twelve for sixteen rows (170
-// registers a thread); fewer where the rings of larger records leave no room.
-template <int D, int NG, int NT>
+// Eights of query rows of an item.  Sixteen rows unpack the codes half as often, but leave a warp
+// its accumulators only at twelve warps an SM: 54 us against 44 us for two items of eight (16
+// requests of 500 to 6000 tokens, 16 rows on 8 KV heads), 84 against 62 us at 24 rows.
+constexpr int NT = 1;
+// Warps of a CTA, two CTAs on an SM; fewer where eight rings of larger records leave no room.
+template <int D, int NG>
 constexpr int warps() {
-  return NT == 2 ? (D == 128 && NG == 4 ? 10 : D == 128 && NG == 2 ? 11 : 12) : D == 128 ? (NG == 4 ? 6 : NG == 2 ? 7 : 8) : 8;
+  return D == 128 ? (NG == 4 ? 6 : NG == 2 ? 7 : 8) : 8;
 }
 // Ring stages of a warp, about 9 KB.
 template <int D>
@@ -132,7 +139,7 @@ constexpr int ring_bytes() {
 }
 // A warp's part of an item as floats: its outputs by column, padded by four floats so that the
 // float4 stores of a quarter-warp (four columns, two dim groups) meet eight different bank groups.
-template <int D, int NT>
+template <int D>
 constexpr int part_floats() {
   return 8 * NT * (D + 4);
 }
@@ -142,9 +149,9 @@ template <int NG>
 constexpr int param_bytes() {
   return kTile * NG * 24;
 }
-template <int D, int NG, int NT>
+template <int D, int NG>
 constexpr int smem_bytes() {
-  return warps<D, NG, NT>() * (ring_bytes<D, NG>() + part_floats<D, NT>() * 4 + param_bytes<NG>());
+  return warps<D, NG>() * (ring_bytes<D, NG>() + part_floats<D>() * 4 + param_bytes<NG>());
 }
 
 // What the join needs to know of a warp's part of an item.
@@ -153,15 +160,15 @@ struct PartInfo {
   int n_tiles, row0, start, n, head0;
 };
 
-template <typename T, int D, int NG, int NT>
-__global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     kv4_attn_split_kernel(const Kv4AttnParams p) {
-  constexpr int WARPS = warps<D, NG, NT>(), THREADS = WARPS * 32;
+  constexpr int WARPS = warps<D, NG>(), THREADS = WARPS * 32;
   constexpr int ROWS = 8 * NT;           // query rows of an item
   constexpr int REC = kv4_record_bytes(D, NG), kStages = stages<D>();
   constexpr int NW = D / 32;             // 32-dim blocks: words per lane and key row
   constexpr int WPG = NW / NG;           // words of one scale group
-  constexpr int PART = part_floats<D, NT>();
+  constexpr int PART = part_floats<D>();
   static_assert(PART * 4 <= ring_bytes<D, NG>(), "a part fits the ring");
   using Work = Kv4Work<ROWS, kTile, THREADS, WARPS, 0>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -731,35 +738,34 @@ __global__ void __launch_bounds__(warps<D, NG, NT>() * 32, NT == 1 ? 2 : 1)
   }
 }
 
-template <typename T, int D, int NG, int NT>
+template <typename T, int D, int NG>
 cudaError_t launch_one(const Kv4AttnParams& p, int sms, bool pdl, cudaStream_t stream) {
-  constexpr int smem = smem_bytes<D, NG, NT>();
-  const auto kernel = kv4_attn_split_kernel<T, D, NG, NT>;
+  constexpr int smem = smem_bytes<D, NG>();
+  const auto kernel = kv4_attn_split_kernel<T, D, NG>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  const int grid = sms * (NT == 1 ? 2 : 1) < kKv4MaxGrid ? sms * (NT == 1 ? 2 : 1) : kKv4MaxGrid;
-  return kv4_launch(kernel, dim3((unsigned)grid), warps<D, NG, NT>() * 32, smem, pdl, stream, p);
+  const int grid = 2 * sms < kKv4MaxGrid ? 2 * sms : kKv4MaxGrid;
+  return kv4_launch(kernel, dim3((unsigned)grid), warps<D, NG>() * 32, smem, pdl, stream, p);
 }
 
-template <typename T, int NT>
-cudaError_t launch_nt(const Kv4AttnParams& p, int sms, bool pdl, cudaStream_t stream) {
+template <typename T>
+cudaError_t launch_t(const Kv4AttnParams& p, int sms, bool pdl, cudaStream_t stream) {
   const int ng = p.c.D / p.c.group;
   if (p.c.D == 128) {
-    if (ng == 1) return launch_one<T, 128, 1, NT>(p, sms, pdl, stream);
-    if (ng == 2) return launch_one<T, 128, 2, NT>(p, sms, pdl, stream);
-    return launch_one<T, 128, 4, NT>(p, sms, pdl, stream);
+    if (ng == 1) return launch_one<T, 128, 1>(p, sms, pdl, stream);
+    if (ng == 2) return launch_one<T, 128, 2>(p, sms, pdl, stream);
+    return launch_one<T, 128, 4>(p, sms, pdl, stream);
   }
-  if (ng == 1) return launch_one<T, 64, 1, NT>(p, sms, pdl, stream);
-  return launch_one<T, 64, 2, NT>(p, sms, pdl, stream);
+  if (ng == 1) return launch_one<T, 64, 1>(p, sms, pdl, stream);
+  return launch_one<T, 64, 2>(p, sms, pdl, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int row_blocks8, int sms, bool bf16, bool pdl,
-                                  cudaStream_t stream) {
-  if (row_blocks8 == 1)
-    return bf16 ? launch_nt<__nv_bfloat16, 1>(p, sms, pdl, stream) : launch_nt<__half, 1>(p, sms, pdl, stream);
-  return bf16 ? launch_nt<__nv_bfloat16, 2>(p, sms, pdl, stream) : launch_nt<__half, 2>(p, sms, pdl, stream);
+int64_t kv4_split_partial_bytes(int D) { return (int64_t)2 * kKv4MaxGrid * 8 * NT * (D + 2) * 4; }
+
+cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int sms, bool bf16, bool pdl, cudaStream_t stream) {
+  return bf16 ? launch_t<__nv_bfloat16>(p, sms, pdl, stream) : launch_t<__half>(p, sms, pdl, stream);
 }
 
 }  // namespace fqkv
