@@ -288,6 +288,27 @@ def test_empty_requests_and_queries_before_the_cache():
     b.check(out)
 
 
+@pytest.mark.parametrize("new", [3, 40, 300])
+def test_refused_requests_give_zeros(new):
+    """seq_lens 0 with queries, as the plan leaves a request that it refuses, beside others."""
+    b = Batch([0, 300, 0, new], [new, 1, 7, new], 8, 2, 128, 128, 16, torch.bfloat16, seed=new)
+    b.fill()
+    out = b.call()
+    assert not out[:new].any() and not out[new + 1:new + 8].any()
+    b.check(out)
+
+
+def test_negative_scale_and_many_requests():
+    """More requests than threads of a block, of one to three tokens; scores times a negative number."""
+    rng = random.Random(5)
+    total = [rng.randint(0, 40) for _ in range(700)]
+    new = [min(t, rng.randint(0, 3)) for t in total]
+    b = Batch(total, new, 4, 1, 64, 64, 16, torch.float16, seed=8)
+    b.fill()
+    b.check(scale=-0.05)
+    b.check(scale=-0.05, max_query_len=1000)
+
+
 @pytest.mark.parametrize("new", [4, 40, 200])
 def test_nan_and_infinity_stay_where_they_are_seen(new):
     """A NaN key, an infinite value: queries before them are exact, queries after them are NaN."""

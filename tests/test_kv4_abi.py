@@ -53,6 +53,9 @@ def attention(cache=None, **kw):
     ({}, dict(bound=-1), _lib.ERR_SHAPE),
     ({}, dict(window=-1), _lib.ERR_SHAPE),
     ({}, dict(stride=8), _lib.ERR_SHAPE),
+    ({}, dict(scale=0.0), _lib.ERR_SHAPE),
+    ({}, dict(scale=float("nan")), _lib.ERR_SHAPE),
+    ({}, dict(scale=float("inf")), _lib.ERR_SHAPE),
     ({}, dict(o_t=1000), _lib.ERR_SHAPE),
     ({}, dict(q_h=-128), _lib.ERR_SHAPE),
     ({}, dict(q=2 * A + 2), _lib.ERR_ALIGN),
