@@ -45,6 +45,26 @@ int check_flags(int64_t flags) {
 
 int done(cudaError_t e, const char* what) { return e == cudaSuccess ? 0 : api_cuda_fail(e, what); }
 
+// n int32 words at p.  The plan's blocks of threads read lengths, free list and count while others
+// write outputs and table entries, so none of what is written may overlap anything else.
+struct Words {
+  const int32_t* p;
+  int64_t n;
+};
+
+bool overlap(const Words& a, const Words& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.n > 0 && b.n > 0 && x < y + 4 * (uintptr_t)b.n && y < x + 4 * (uintptr_t)a.n;
+}
+
+// Whether `a` meets the first `width` words of one of `rows` rows, `stride` words apart.
+bool overlap_rows(const Words& a, const int32_t* rows_at, int64_t rows, int64_t stride, int64_t width) {
+  if (width <= 0 || !overlap(a, Words{rows_at, (rows - 1) * stride + width})) return false;
+  const int64_t x = reinterpret_cast<intptr_t>(a.p) - reinterpret_cast<intptr_t>(rows_at);
+  if (x < 0 || x % (4 * stride) < 4 * width) return true;
+  return x / (4 * stride) + 1 < rows && x + 4 * a.n > (x / (4 * stride) + 1) * 4 * stride;
+}
+
 bool for_prompts(int64_t G, int64_t max_query_len) { return max_query_len > kPromptRows / G; }
 
 }  // namespace
@@ -68,8 +88,18 @@ extern "C" FQKV_API int fqkv_kv4_plan(const int32_t* context_lens, const int32_t
     return api_fail(FQKV_ERR_SHAPE, "block_size must be a positive multiple of 16");
   if (table_width < 0 || table_width > INT32_MAX || table_stride < table_width)
     return api_fail(FQKV_ERR_SHAPE, "table_stride must be at least table_width, which is not negative");
-  if (n_free == n_free_out)
-    return api_fail(FQKV_ERR_ALIAS, "n_free_out must not be n_free: every CTA reads n_free");
+  const Words words[] = {{query_start, n_requests + 1}, {positions, n_tokens},     {slots, n_tokens},
+                         {seq_lens, n_requests},        {n_free_out, 1},           {refused, 1},  // six written
+                         {context_lens, n_requests},    {new_lens, n_requests},    {free_blocks, free_capacity},
+                         {n_free, 1}};
+  for (int i = 0; i < 10; ++i) {
+    if (overlap_rows(words[i], block_tables, n_requests, table_stride, table_width))
+      return api_fail(FQKV_ERR_ALIAS, "block_tables, which the plan writes, overlaps another argument");
+    for (int j = i < 6 ? i + 1 : 10; j < 10; ++j)
+      if (overlap(words[i], words[j]))
+        return api_fail(FQKV_ERR_ALIAS, "an output of the plan overlaps an input or another output: every CTA reads all "
+                                        "lengths, the free list and n_free");
+  }
   if (int rc = check_flags(flags)) return rc;
   int sms = 0;
   if (int rc = api_sm100(&sms)) return rc;

@@ -172,8 +172,9 @@ def kv4_plan(
             (pass ``plan.n_free`` on to the next step).
         block_size: tokens per block.
         n_tokens: tokens of the batch (or an upper bound; surplus tokens get slot -1).
-        out: a ``KV4Plan`` of the same sizes to write into (its ``n_free`` must not be the
-            ``n_free`` passed in).
+        out: a ``KV4Plan`` of the same sizes to write into.  None of its tensors may overlap
+            another argument (lengths cannot be updated in place: every block of threads reads
+            them all).
 
     A request whose blocks do not fit the table, whose tokens do not fit ``n_tokens`` or that
     the free list cannot serve is refused: no blocks, ``seq_lens`` 0, slots -1.

@@ -291,7 +291,8 @@ FQKV_API int64_t fqkv_kv4_record_bytes(int64_t head_dim, int64_t group_size);
  *   query_start [R + 1]  first token of each request (clipped to n_tokens)
  *   positions, slots [n_tokens]  0 and -1 past the last request's tokens
  *   seq_lens [R]  context + new, or 0;  n_free_out [1];  refused [1]
- * All int32.  A negative length counts as 0 tokens and is refused.
+ * All int32.  A negative length counts as 0 tokens and is refused.  What is written (the six
+ * outputs and block_tables) must overlap no input and nothing else that is written: FQKV_ERR_ALIAS.
  */
 FQKV_API int fqkv_kv4_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t n_requests,
                 int32_t* block_tables, int64_t table_stride, int64_t table_width,
