@@ -52,6 +52,7 @@ struct Kv4Work {
     long long found[POINTS], per_head[POINTS];
     Kv4Request req[POINTS];
     int r[POINTS];
+    int rows[2];  // tokens of the batch that belong to a request: [rows[0], rows[1])
   };
 
   long long total, u0, u1;  // all tiles, this CTA's run
@@ -120,12 +121,20 @@ struct Kv4Work {
     return sum;
   }
 
+  // Zeros for tokens [lo, hi) of out, which no item holds.
+  static __device__ __forceinline__ void zero_rows(const Kv4AttnParams& p, int64_t lo, int64_t hi) {
+    for (int64_t t = lo + blockIdx.x; t < hi; t += gridDim.x)
+      for (int e = threadIdx.x; e < p.n_q * p.c.D / 8; e += THREADS)
+        reinterpret_cast<uint4*>(p.out + t * p.o_t)[e] = make_uint4(0, 0, 0, 0);
+  }
+
   // First tile of the run of point k.
   __device__ __forceinline__ long long point(int k) const {
     return POINTS == 1 ? u0 : u0 + kv4_muldiv(k, u1 - u0, POINTS, small);
   }
 
-  // Called by the whole block.  False: this CTA has no work.
+  // Called by the whole block.  False: this CTA has no work.  Tokens of no request (a plan's upper
+  // bound of the tokens leaves some past the last request's) are written here, without any work too.
   __device__ __forceinline__ bool locate(const Kv4AttnParams& p, Shared& s, int max_ctas, int min_tiles) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Kv4Request none{0, 0, 0};
@@ -138,6 +147,8 @@ struct Kv4Work {
     for (int k0 = 0; k0 < p.R; k0 += THREADS) {
       const int k = k0 + tid;
       q = k < p.R ? kv4_load_request(p, k) : none;
+      if (k == 0) s.rows[0] = q.start;
+      if (k == p.R - 1) s.rows[1] = q.start + q.n;
       heads = head_tiles(p, q);
       long long v = heads * p.c.n_kv;
 #pragma unroll
@@ -154,6 +165,10 @@ struct Kv4Work {
         total += s.scan[w];
       }
       if (!one) __syncthreads();
+    }
+    if (p.query_start) {
+      zero_rows(p, 0, s.rows[0]);
+      zero_rows(p, s.rows[1], p.T);
     }
     ctas = (int)max(1ll, min((long long)max_ctas, total / min_tiles));
     small = total < (1ll << 32) / 1024;

@@ -289,7 +289,8 @@ def kv4_attention(
 
     Returns:
         (tokens, n_q_heads, D) in the cache's dtype, (B, S, n_q_heads, D) for a head-major ``q``:
-        rows ready for the output projection.  A query that sees nothing gives zeros.
+        rows ready for the output projection.  A query that sees nothing gives zeros, and so does a
+        token of no request (before ``query_start[0]`` or from ``query_start[R]`` on).
     """
     assert q.is_cuda, "kv4_attention requires CUDA tensors"
     D, index = cache.head_dim, cache.index
@@ -342,7 +343,7 @@ def kv4_attention(
             raise ValueError("out's heads must be contiguous")
         o_t = rows.stride(0) if T > 1 else n_q * D
     if T == 0 or R == 0:
-        return out
+        return out.zero_()
     key = (n_q, cache.n_kv_heads, D, min(bound, _SPLIT_MAX_ROWS + 1))
     need = _workspace.get(key)
     if need is None:

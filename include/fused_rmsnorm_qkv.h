@@ -325,7 +325,8 @@ FQKV_API int fqkv_kv4_gather(const fqkv_kv4_cache* cache, const int32_t* slots, 
  * Causal attention of the batch's new tokens over the cache (their own keys and values
  * already appended).  Request r has n = query_start[r + 1] - query_start[r] queries (n_seq
  * each when query_start is NULL); its query j sees tokens t <= p and, with window > 0,
- * t > p - window, where p = seq_lens[r] - n + j.  A query that sees nothing gives zeros.
+ * t > p - window, where p = seq_lens[r] - n + j.  A query that sees nothing gives zeros, as does
+ * a token before query_start[0] or from query_start[R] on.
  *   q    request r, query j, head h at r * q_stride_r + j * q_stride_t + h * q_stride_h, or,
  *        with query_start, token query_start[r] + j in the place of both; 16-byte aligned rows
  *   out  [n_tokens, n_q_heads, head_dim] in the cache's dtype, row stride out_stride_t

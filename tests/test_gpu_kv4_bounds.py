@@ -1,0 +1,86 @@
+"""The paged 4-bit cache where it can go wrong: tokens of no request, block ids that name no slot,
+groups of very different size, one key that outweighs a long tail, NaN values whose weight
+underflows, numbers at the end of the 16-bit range, windows of the largest integer and refused
+requests that are tried again.  The bounds are those of test_gpu_kv4.py, applied group by group
+where the groups differ; fp16 outputs below 2^-14 add half of the subnormal step, 2^-25."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv4 as ref
+from test_gpu_kv4 import DT, U, Batch, heads, i32
+from triton_fused_rmsnorm_qkv import device_status, kv4_append, kv4_attention, kv4_cache, kv4_plan
+
+pytestmark = pytest.mark.gpu
+IDS = ["bf16", "fp16"]
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    yield
+    assert device_status() == 0
+
+
+def check_groups(b, group, got=None, **kw):
+    """``Batch.check`` for each group of dims by itself."""
+    got = (b.call(**kw) if got is None else got).cpu().double()
+    kw.pop("max_query_len", None)
+    want, spread = b.reference(**kw)
+    u, tiny = U[b.dtype], 2.0 ** -25 if b.dtype == torch.float16 else 1e-30
+    for at in range(0, want.shape[-1], group):
+        g, w, s = (x[..., at:at + group] for x in (got, want, spread))
+        bound = 8 * u * torch.maximum(w.abs(), s) + tiny
+        assert ((g - w).abs() <= bound).all(), (at, ((g - w).abs() / bound).max())
+        assert (g - w).norm() <= 1.5 * u * w.norm() + tiny * math.sqrt(w.numel()), (at, (g - w).norm() / w.norm() / u)
+
+
+# ------------------------------------------------------------------ tokens of no request
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 0], [40, 1, 90], [0, 0, 0]])
+def test_tokens_of_no_request_are_zeros(new, dtype):
+    """Tokens before the first request's and past the last one's, as a plan with an upper bound of
+    the tokens leaves them: zeros in both kernels, whatever `out` held, also without any query."""
+    b = Batch([max(n, 1) + 60 for n in new], new, 8, 2, 128, 64, 16, dtype, seed=len(new))
+    b.fill()
+    before, after = 2, 301
+    q = torch.cat([heads(9, before, 8, 128, dtype=dtype), b.q, heads(8, after, 8, 128, dtype=dtype)]).cuda()
+    start = i32([before + s for s in b.start])
+    for bound in (1, q.shape[0]):
+        wide = torch.full((q.shape[0], 9, 128), math.nan, dtype=dtype, device="cuda")
+        for out in (torch.full_like(q, math.nan), wide[:, :8]):
+            kv4_attention(q, b.cache, i32(b.tables), i32(b.total), start, max_query_len=bound, out=out)
+            assert not out[:before].any() and not out[before + b.start[-1]:].any()
+            if b.start[-1]:
+                b.check(out[before:before + b.start[-1]])
+        assert wide[:, 8].isnan().all()
+
+
+def test_no_requests_give_zeros():
+    b = Batch([40], [1], 8, 2, 128, 128, 16, torch.bfloat16)
+    q = heads(1, 5, 8, 128).cuda()
+    out = torch.full_like(q, math.nan)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    kv4_attention(q, b.cache, torch.zeros(0, 3, dtype=torch.int32, device="cuda"), none, i32([0]), out=out)
+    assert not out.any()
+
+
+def test_a_padded_step_of_a_plan():
+    """A plan whose token count is an upper bound, through append and attention."""
+    n_kv, D, block, T = 2, 64, 16, 24
+    cache = kv4_cache(8, n_kv, D, block_size=block)
+    tables = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
+    plan = kv4_plan(i32([0, 0]), i32([5, 9]), tables, torch.randperm(8, device="cuda").int(), i32([8]), block_size=block,
+                    n_tokens=T)
+    k, v, q = (heads(s, T, h, D) for s, h in ((1, n_kv), (2, n_kv), (3, 8)))
+    kv4_append(cache, k.cuda(), v.cuda(), plan.slots)
+    out = torch.full((T, 8, D), math.nan, dtype=q.dtype, device="cuda")
+    kv4_attention(q.cuda(), cache, tables, plan.seq_lens, plan.query_start, max_query_len=9, out=out)
+    assert not out[14:].any()
+    kk, vv = (ref.values(*ref.quantise(x, D)) for x in (k, v))
+    for lo, hi in ((0, 5), (5, 14)):
+        want, spread = ref.attention(q[lo:hi].double(), kk[lo:hi], vv[lo:hi], hi - lo)
+        got = out[lo:hi].cpu().double()
+        assert ((got - want).abs() <= 8 * U[q.dtype] * torch.maximum(want.abs(), spread)).all()
