@@ -112,7 +112,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const Kv4PlanPar
           block = p.free_blocks[n_free - 1 - (before + (nth - s_have[a]))];
           if (in_block == 0) *entry = block;
         }
-        slot = block * p.P + in_block;
+        // An id without a slot (negative, or past what 31 bits name) stores nothing.
+        const long long at = (long long)block * p.P + in_block;
+        if (at < 0 || at > INT32_MAX) record_status(FQKV_STATUS_BAD_INDEX);
+        else slot = (int)at;
       }
       p.positions[t] = pos;
       p.slots[t] = slot;

@@ -290,6 +290,8 @@ FQKV_API int64_t fqkv_kv4_record_bytes(int64_t head_dim, int64_t group_size);
  * request that is not granted takes no blocks, has seq_lens 0 and slots -1, and is counted.
  *   query_start [R + 1]  first token of each request (clipped to n_tokens)
  *   positions, slots [n_tokens]  0 and -1 past the last request's tokens
+ *        (a block id that is negative or whose slot passes 2^31 - 1 gives slot -1 and
+ *        FQKV_STATUS_BAD_INDEX; ids past the cache are reported where they are used)
  *   seq_lens [R]  context + new, or 0;  n_free_out [1];  refused [1]
  * All int32.  A negative length counts as 0 tokens and is refused.  What is written (the six
  * outputs and block_tables) must overlap no input and nothing else that is written: FQKV_ERR_ALIAS.

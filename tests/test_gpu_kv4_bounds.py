@@ -84,3 +84,21 @@ def test_a_padded_step_of_a_plan():
         want, spread = ref.attention(q[lo:hi].double(), kk[lo:hi], vv[lo:hi], hi - lo)
         got = out[lo:hi].cpu().double()
         assert ((got - want).abs() <= 8 * U[q.dtype] * torch.maximum(want.abs(), spread)).all()
+
+
+# ------------------------------------------------------------------ block ids that name no slot
+@pytest.mark.parametrize("bad", [-1, -(2 ** 31), 1 << 27, 1 << 28, 2 ** 31 - 1])
+def test_plan_reports_blocks_without_a_slot(bad):
+    """A held block, and a block of the free list, whose id is negative or whose slots pass 2^31."""
+    plan = kv4_plan(i32([3, 20]), i32([2, 2]), i32([[bad, -1], [5, 6]]), i32([7]), i32([1]), block_size=16, n_tokens=4)
+    assert device_status() == 2
+    assert plan.slots.tolist() == [-1, -1, 6 * 16 + 4, 6 * 16 + 5] and plan.positions.tolist() == [3, 4, 20, 21]
+    plan = kv4_plan(i32([3, 15]), i32([2, 2]), i32([[1, -1], [5, -1]]), i32([bad]), i32([1]), block_size=16, n_tokens=4)
+    assert device_status() == 2
+    assert plan.slots.tolist() == [19, 20, 5 * 16 + 15, -1] and plan.seq_lens.tolist() == [5, 17]
+
+
+def test_plan_takes_the_last_block_with_a_slot():
+    last = (2 ** 31 - 1) // 16 - 1   # its last slot is below 2^31 - 1
+    plan = kv4_plan(i32([15]), i32([1]), i32([[last]]), i32([0]), i32([0]), block_size=16, n_tokens=1)
+    assert plan.slots.tolist() == [last * 16 + 15]
