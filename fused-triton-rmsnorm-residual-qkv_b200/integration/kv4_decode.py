@@ -51,7 +51,7 @@ class PagedKV4Decoder:
         core = self.model.model
         plan = kv4_plan(self.lens, self.ones if S == 1 else torch.full_like(self.lens, S), self.tables, self.free,
                         self.n_free, block_size=self.block_size, n_tokens=B * S)
-        self.lens.copy_(plan.seq_lens)
+        plan.context_after(self.lens, out=self.lens)
         self.n_free.copy_(plan.n_free)
         x, residual = core.embed_tokens(ids), None
         cos, sin = core.rotary_emb(x, plan.positions.view(B, S).long())
@@ -60,7 +60,7 @@ class PagedKV4Decoder:
             q, k, v, hidden = fused_add_rmsnorm_qkv_rope(x, residual, norm.weight, weight, cos, sin, self.n_q, self.n_kv,
                                                          self.head_dim, norm.variance_epsilon)
             kv4_append(cache, k, v, plan.slots)
-            out = kv4_attention(q, cache, self.tables, self.lens, scale=layer.self_attn.scaling)
+            out = kv4_attention(q, cache, self.tables, plan.seq_lens, scale=layer.self_attn.scaling)
             residual = hidden + layer.self_attn.o_proj(out.reshape(B, S, -1))
             x = layer.mlp(layer.post_attention_layernorm(residual))
         return self.model.lm_head(core.norm((x + residual)[:, -1:]))[:, 0]

@@ -7,7 +7,8 @@ groups of 128) in blocks that requests own through block tables, and attend over
 
     plan = kv4_plan(context_lens, new_lens, block_tables, free_blocks, n_free, ...)
     kv4_append(cache, k, v, plan.slots)
-    out = kv4_attention(q, cache, block_tables, plan.seq_lens, plan.query_start)
+    out = kv4_attention(q, cache, block_tables, plan.seq_lens, plan.query_start, max_query_len=longest)
+    context_lens, n_free = plan.context_after(context_lens), plan.n_free   # of the next step
 
 A cached number is ``scale * code + minimum`` with ``minimum = min(x)``, ``scale`` the group's
 ``(max - min) * (1/15)`` rounded to the cache's dtype and ``code = rint((x - minimum) / scale)``
@@ -83,6 +84,11 @@ class KV4Plan(NamedTuple):
     seq_lens: torch.Tensor     # (R,) context + new tokens, or 0 for a refused request
     n_free: torch.Tensor       # (1,) free blocks left
     refused: torch.Tensor      # (1,) requests that were not granted
+
+    def context_after(self, context_lens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next step's ``context_lens``: ``seq_lens`` of a granted request, the context of a
+        refused one, which keeps its tokens and blocks.  ``out`` may be ``context_lens``."""
+        return torch.maximum(context_lens, self.seq_lens, out=out)
 
 
 def kv4_record_bytes(head_dim: int, group_size: int) -> int:
@@ -177,7 +183,9 @@ def kv4_plan(
             them all).
 
     A request whose blocks do not fit the table, whose tokens do not fit ``n_tokens`` or that
-    the free list cannot serve is refused: no blocks, ``seq_lens`` 0, slots -1.
+    the free list cannot serve is refused: no blocks, ``seq_lens`` 0, slots -1.  It can be tried
+    again in a later step: ``plan.context_after(context_lens)`` holds what it had (``seq_lens`` as the
+    next step's context would start it from nothing, over its own blocks).
     """
     assert context_lens.is_cuda, "kv4_plan requires CUDA tensors"
     index, R = context_lens.get_device(), context_lens.numel()

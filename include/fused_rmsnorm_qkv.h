@@ -288,6 +288,7 @@ FQKV_API int64_t fqkv_kv4_record_bytes(int64_t head_dim, int64_t group_size);
  * A request is granted when its blocks fit the table's width, its tokens end within n_tokens,
  * and it needs no block or the blocks needed up to and including it are at most n_free.  A
  * request that is not granted takes no blocks, has seq_lens 0 and slots -1, and is counted.
+ * It keeps its tokens and blocks: the next step's context is max(context_lens, seq_lens).
  *   query_start [R + 1]  first token of each request (clipped to n_tokens)
  *   positions, slots [n_tokens]  0 and -1 past the last request's tokens
  *        (a block id that is negative or whose slot passes 2^31 - 1 gives slot -1 and

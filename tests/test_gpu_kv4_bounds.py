@@ -102,3 +102,54 @@ def test_plan_takes_the_last_block_with_a_slot():
     last = (2 ** 31 - 1) // 16 - 1   # its last slot is below 2^31 - 1
     plan = kv4_plan(i32([15]), i32([1]), i32([[last]]), i32([0]), i32([0]), block_size=16, n_tokens=1)
     assert plan.slots.tolist() == [last * 16 + 15]
+
+
+# ------------------------------------------------------------------ refused requests
+def test_a_refused_request_keeps_its_history():
+    """Request 1 needs a block while none is free: it stores nothing and keeps its tokens and blocks.
+    The step after, with a block given back, continues where it was."""
+    n_q, n_kv, D, block = 4, 2, 64, 16
+    cache = kv4_cache(5, n_kv, D, block_size=block)
+    cache.data.fill_(255)
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    free, n_free = i32([3, 0, 4, 1, 2]), i32([5])
+    ctx = i32([0, 0, 0])
+    past_k, past_v = [[], [], []], [[], [], []]
+    #        (new tokens, refused, lengths after)
+    steps = [([33, 16, 2], 0, [33, 16, 2]), ([1, 1, 1], 1, [34, 16, 3]), ([1, 1, 0], 0, [35, 17, 0])]
+    for step, (new, refused, after) in enumerate(steps):
+        T = sum(new)
+        if step == 2:    # request 2 is finished: its block is free again
+            blocks = tables.cpu()
+            assert blocks[1, 0] >= 0 and blocks[1, 1] == -1
+            free, n_free, ctx = tables[2, :1].clone(), i32([1]), ctx * i32([1, 1, 0])
+            tables[2] = -1
+        plan = kv4_plan(ctx, i32(new), tables, free, n_free, block_size=block, n_tokens=T)
+        k, v, q = (heads(10 * step + s, T, h, D) for s, h in ((1, n_kv), (2, n_kv), (3, n_q)))
+        kv4_append(cache, k.cuda(), v.cuda(), plan.slots)
+        out = kv4_attention(q.cuda(), cache, tables, plan.seq_lens, plan.query_start, max_query_len=max(new)).cpu()
+        assert plan.refused.item() == refused
+        lens, at = plan.seq_lens.tolist(), 0
+        for r, n in enumerate(new):
+            if n and lens[r] == 0:
+                assert not out[at:at + n].any()
+            elif n:
+                past_k[r].append(k[at:at + n])
+                past_v[r].append(v[at:at + n])
+                kk, vv = (ref.values(*ref.quantise(torch.cat(x[r]), D)) for x in (past_k, past_v))
+                want, spread = ref.attention(q[at:at + n].double(), kk, vv, n)
+                err = (out[at:at + n].double() - want).abs()
+                assert (err <= 8 * U[q.dtype] * torch.maximum(want.abs(), spread)).all()
+            at += n
+        ctx, n_free = plan.context_after(ctx), plan.n_free
+        assert ctx.tolist() == after
+    held = [x for row in tables.tolist() for x in row if x >= 0]
+    assert len(held) == len(set(held)) == 5
+
+
+def test_context_after_in_place():
+    tables = i32([[0, -1], [1, -1], [2, -1]])
+    ctx = i32([5, 16, 3])
+    plan = kv4_plan(ctx, i32([2, 1, 0]), tables, i32([3]), i32([0]), block_size=16, n_tokens=3)
+    assert plan.seq_lens.tolist() == [7, 0, 3]
+    assert plan.context_after(ctx, out=ctx) is ctx and ctx.tolist() == [7, 16, 3]
