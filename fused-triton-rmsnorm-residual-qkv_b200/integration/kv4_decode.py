@@ -29,6 +29,9 @@ class PagedKV4Decoder:
         self.n_q, self.n_kv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.head_dim = core.layers[0].self_attn.head_dim
         self.block_size = block_size
+        if any(getattr(layer.self_attn, name).bias is not None for layer in core.layers
+               for name in ("q_proj", "k_proj", "v_proj")):
+            raise ValueError("the fused projection has no bias: the model's q_proj, k_proj and v_proj must not have one")
         self.qkv_weights = [pack_qkv_weight(layer.self_attn) for layer in core.layers]
         self.width = -(-max_len // block_size)
         dtype = self.qkv_weights[0].dtype

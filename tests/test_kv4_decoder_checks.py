@@ -1,0 +1,24 @@
+"""``PagedKV4Decoder`` refuses what it does not compute, before any kernel runs.  CPU only."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from integration import PagedKV4Decoder
+from transformers import LlamaConfig, LlamaForCausalLM
+
+
+def _model(**kw):
+    return LlamaForCausalLM(LlamaConfig(hidden_size=128, intermediate_size=64, num_hidden_layers=2, num_attention_heads=2,
+                                        num_key_value_heads=1, head_dim=64, vocab_size=32, **kw)).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("only", ["q_proj", "k_proj", "v_proj"])
+def test_attention_bias_is_refused(only):
+    model = _model(attention_bias=True)
+    for layer in model.model.layers:
+        for name in ("q_proj", "k_proj", "v_proj"):
+            if name != only:
+                getattr(layer.self_attn, name).bias = None
+    with pytest.raises(ValueError, match="bias"):
+        PagedKV4Decoder(model, 1, 32)
