@@ -68,9 +68,19 @@ class PagedKV4Decoder:
             x = layer.mlp(layer.post_attention_layernorm(residual))
         return self.model.lm_head(core.norm((x + residual)[:, -1:]))[:, 0]
 
+    def _check(self, prompt: torch.Tensor, room: int, wanted: int) -> None:
+        """The prompt and ``room`` tokens after it must fit, and something must be asked for."""
+        B, P = prompt.shape
+        if B != self.batch or P == 0 or wanted <= 0 or P + room > self.max_len:
+            raise ValueError(f"prompt {tuple(prompt.shape)} + {room} tokens does not fit batch {self.batch}, "
+                             f"max_len {self.max_len}")
+
     @torch.no_grad()
     def forced_logits(self, prompt: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
         """Teacher forcing, eagerly: the fp32 logits that predict ``tokens[:, t]`` for every t."""
+        self._check(prompt, tokens.shape[1] - 1, tokens.shape[1])
+        if tokens.shape[0] != self.batch:
+            raise ValueError(f"tokens {tuple(tokens.shape)} do not follow {self.batch} prompts")
         self._reset()
         logits = [self._forward(prompt).float()]
         for t in range(tokens.shape[1] - 1):
@@ -81,10 +91,7 @@ class PagedKV4Decoder:
     def generate(self, prompt: torch.Tensor, n_new: int) -> torch.Tensor:
         """The ``n_new`` greedy tokens after ``prompt`` (batch, P): the prompt and the first step
         run eagerly, every later step is a replay of one captured graph."""
-        B, P = prompt.shape
-        if B != self.batch or P + n_new > self.max_len:
-            raise ValueError(f"prompt {tuple(prompt.shape)} + {n_new} tokens does not fit batch {self.batch}, "
-                             f"max_len {self.max_len}")
+        self._check(prompt, n_new, n_new)
         self._reset()
         tok = self._forward(prompt).argmax(-1, keepdim=True)
         tokens = [tok.clone()]

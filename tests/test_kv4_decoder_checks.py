@@ -22,3 +22,17 @@ def test_attention_bias_is_refused(only):
                 getattr(layer.self_attn, name).bias = None
     with pytest.raises(ValueError, match="bias"):
         PagedKV4Decoder(model, 1, 32)
+
+
+def test_sequences_past_the_cache_are_refused():
+    """Teacher forcing appends the prompt and all forced tokens but the last."""
+    dec = object.__new__(PagedKV4Decoder)
+    dec.batch, dec.max_len = 2, 16
+    ids = torch.zeros(2, 12, dtype=torch.long)
+    for prompt, tokens in ((ids, ids[:, :6]), (ids[:1], ids[:1, :2]), (ids, ids[:1, :2]), (ids[:, :0], ids[:, :2]),
+                           (ids, ids[:, :0])):
+        with pytest.raises(ValueError):
+            dec.forced_logits(prompt, tokens)
+    for prompt, n_new in ((ids, 5), (ids[:1], 1), (ids[:, :0], 3), (ids, 0)):
+        with pytest.raises(ValueError):
+            dec.generate(prompt, n_new)
