@@ -10,9 +10,10 @@
 // cost one shift and four three-input logic operations.  For the keys the constants are taken back
 // by the value the accumulator starts with; for the values they are subtracted and the codes
 // centred, so that the sum over a long context does not cancel a large offset.  bf16 queries are
-// divided by a power of two per row and the weights p s are held at 1 or less by the reference
-// exponent, so fp16 loses nothing of either range.  p s is rounded to 16 bits for the product (the
-// one rounding to fewer than 32 bits besides the output); maxima, sums and outputs are fp32.
+// divided by a power of two per row.  p s is rounded to 16 bits for the product (the one rounding to
+// fewer than 32 bits besides the output); maxima, sums and outputs are fp32.  The reference exponent
+// holds the largest p s at 2^15, near the end of fp16's range, so that a weight keeps its eleven bits
+// down to 2^-29 of the largest and is dropped below 2^-40 of it (2^20 such weights are 2^-20 of it).
 //
 // Shape.  Both products are transposed (keys x queries and dims x queries, m16n8k16), so the
 // query heads that share a KV head fill the 8-wide side and 1 to 8 query rows cost the same.
@@ -37,6 +38,7 @@ namespace fqkv {
 namespace {
 
 constexpr int kTile = 32;    // tokens per ring stage (two records)
+constexpr float kRoom = 15.0f;  // log2 of the largest weight p s
 
 // Untiled bulk copy global -> shared, counted on a local mbarrier.  Addresses and size are
 // multiples of 16 bytes.
@@ -383,8 +385,9 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           if (sv[grp] == 0.0f) sv[grp] = fmaxf(fabsf(mv[grp]), 1e-20f);
           widest = fmaxf(widest, sv[grp]);
         }
-        float lg = log2_approx(widest);
-        if (!(fabsf(lg) < 1e9f)) lg = 0.0f;  // not finite: whoever sees the key becomes NaN
+        // Below 2^-60 a token counts as 2^-60, so that its probability and their sum stay in fp32's range.
+        float lg = fmaxf(log2_approx(widest), -60.0f);
+        if (!(lg < 1e9f)) lg = 0.0f;  // not finite: whoever sees the key becomes NaN
         __syncwarp();                        // the previous tile's have been read
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -455,8 +458,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
               if (!seen) s[m][nt][e] = -INFINITY;
             }
       }
-      // ---- the reference exponent is that of p s, so that the weights p s are at most 1 and fp16
-      // holds them whatever the scales
+      // ---- the reference exponent is that of p s, so that the weights p s are at most 2^kRoom
       float lg[2][2];  // record, key g or g + 8
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];
+        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e] - kRoom;
       // ---- probabilities, and the products with the values
 #pragma unroll
       for (int m = 0; m < 2; ++m) {

@@ -153,3 +153,26 @@ def test_context_after_in_place():
     plan = kv4_plan(ctx, i32([2, 1, 0]), tables, i32([3]), i32([0]), block_size=16, n_tokens=3)
     assert plan.seq_lens.tolist() == [7, 0, 3]
     assert plan.context_after(ctx, out=ctx) is ctx and ctx.tolist() == [7, 16, 3]
+
+
+# ------------------------------------------------------------------ weights of very different size
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("D,group", [(128, 128), (64, 64), (64, 32)])
+def test_a_dominant_key_and_a_long_tail(D, group, dtype):
+    """131071 keys of which one outweighs each of the others by 2^25.2: together they hold 0.34 % of
+    the weight, and their values are three times as large as the one key's.  The requests share
+    their blocks and are so many that a warp walks through two requests' keys."""
+    T, R = 131071, 4736
+    b = Batch([T], [1], 2, 1, D, group, 64, dtype, seed=1)
+    g = torch.Generator().manual_seed(2)
+    b.q = torch.ones(1, 2, D).to(dtype)
+    b.k = torch.zeros(T, 1, D, dtype=dtype)
+    b.k[777] = 25.2 * math.log(2) / math.sqrt(D)
+    b.v = (6.0 + 15 * torch.rand(T, 1, D, generator=g)).to(dtype)
+    b.v[777] = (15 * torch.rand(1, D, generator=g) - 7.5).to(dtype)
+    b.fill()
+    out = kv4_attention(b.q.cuda().expand(R, -1, -1).contiguous(), b.cache, i32(b.tables).repeat(R, 1), i32([T] * R))
+    want, spread = b.reference()
+    err = (out.cpu().double() - want).abs()
+    assert (err <= 8 * U[dtype] * torch.maximum(want.abs(), spread)).all()
+    assert (err.flatten(1).norm(dim=1) <= 1.5 * U[dtype] * want.norm()).all(), err.norm(dim=(1, 2)).max() / want.norm()
