@@ -14,6 +14,8 @@
 // fewer than 32 bits besides the output); maxima, sums and outputs are fp32.  The reference exponent
 // holds the largest p s at 2^15, near the end of fp16's range, so that a weight keeps its eleven bits
 // down to 2^-29 of the largest and is dropped below 2^-40 of it (2^20 such weights are 2^-20 of it).
+// Where a head has several groups, s is in the group's own unit, so "the largest" is the group's own
+// up to what its scales differ from key to key.
 //
 // Shape.  Both products are transposed (keys x queries and dims x queries, m16n8k16), so the
 // query heads that share a KV head fill the 8-wide side and 1 to 8 query rows cost the same.
@@ -39,6 +41,10 @@ namespace {
 
 constexpr int kTile = 32;    // tokens per ring stage (two records)
 constexpr float kRoom = 15.0f;  // log2 of the largest weight p s
+// Several groups in a head have a unit each, a power of two between 2^-60 and 2^60 that keeps the
+// largest of the group's scales so far below 1; it is taken with a factor of four to spare, so that it
+// hardly moves.
+constexpr int kMostUnit = 60, kUnitRoom = 2;
 
 // Untiled bulk copy global -> shared, counted on a local mbarrier.  Addresses and size are
 // multiples of 16 bytes.
@@ -93,6 +99,10 @@ __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& lo, fl
   hi = __uint_as_float(w & 0xFFFF0000u);
 }
 
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+__device__ __forceinline__ float reciprocal_of_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 // a / b by an approximate reciprocal and one step of refinement; exact where the quotient is a
 // small integer.  Not meaningful for b = 0 or subnormal.
 __device__ __forceinline__ float quotient(float a, float b) {
@@ -146,7 +156,7 @@ constexpr int part_floats() {
   return 8 * NT * (D + 4);
 }
 // A stage's parameters as the lanes use them, per token and group: the values' {s, r, z, log2 of
-// the token's largest s}, then the keys' {s, m}.
+// the token's largest s}, s and z in the group's unit, then the keys' {s, m}.
 template <int NG>
 constexpr int param_bytes() {
   return kTile * NG * 24;
@@ -179,6 +189,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
   __shared__ Work s_item[WARPS], s_ahead[WARPS];  // each warp's item, and the item its copies have reached
   __shared__ PartInfo s_info[WARPS][2];
   __shared__ float s_max[WARPS][2][ROWS], s_sum[WARPS][2][ROWS];
+  __shared__ float s_unit[WARPS][NG];  // each warp's powers of two that its groups' scales are multiplied by
   __shared__ int s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -367,6 +378,11 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       }
     }
 
+    if (NG > 1) {
+      __syncwarp();
+      if (lane < NG) s_unit[warp][lane] = power_of_two(kMostUnit);
+      __syncwarp();
+    }
     for (int tile = wt; tile < we; ++tile) {
       mbar_wait(&s_bar[warp][stage], (parity >> stage) & 1u);
       parity ^= 1u << stage;
@@ -377,18 +393,62 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         uint32_t wk[NG], wv[NG];
         lds_words<NG>(at, wk);
         lds_words<NG>(at + 64 * NG, wv);
-        float sv[NG], mv[NG], widest = 0.0f;
-#pragma unroll
-        for (int grp = 0; grp < NG; ++grp) {
+        float sv[NG], mv[NG], unit[NG], widest = 0.0f;
+        const auto scaled = [&](int grp) {
           unpack2<T>(wv[grp], sv[grp], mv[grp]);
           // A scale of zero goes with codes of zero; any scale then stands for the same numbers.
           if (sv[grp] == 0.0f) sv[grp] = fmaxf(fabsf(mv[grp]), 1e-20f);
+          if (NG > 1) sv[grp] *= unit[grp], mv[grp] *= unit[grp];
+        };
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          unit[grp] = NG > 1 ? s_unit[warp][grp] : 1.0f;
+          scaled(grp);
           widest = fmaxf(widest, sv[grp]);
+        }
+        if constexpr (NG > 1) {
+          if (__any_sync(~0u, widest > 1.0f)) {  // what was added up is brought to the new units
+            const Work& x = s_item[warp];
+            const int t = tile * kTile + lane, first = x.req.len - x.req.n;
+            const int j0 = (int)((uint32_t)(x.rb * ROWS) / (uint32_t)p.G);
+            const int j1 = (int)((uint32_t)(x.rb * ROWS + ROWS - 1) / (uint32_t)p.G);
+            // (what no row of the block sees may be anything)
+            const bool visible = t < x.req.len && t <= first + j1 && (p.window <= 0 || t > first + j0 - p.window);
+#pragma unroll
+            for (int grp = 0; grp < NG; ++grp) {
+              const float old = unit[grp];
+              unit[grp] = 1.0f;
+              scaled(grp);
+              // (positive floats are ordered as integers)
+              const uint32_t most = __reduce_max_sync(~0u, visible && sv[grp] < INFINITY ? __float_as_uint(sv[grp]) : 0u);
+              const int up = max(-kMostUnit, min(kMostUnit, 126 - kUnitRoom - (int)(most >> 23)));
+              unit[grp] = fminf(old, power_of_two(up));
+              const float f = unit[grp] * reciprocal_of_power(old);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                bias[0][grp][e] *= f;
+#pragma unroll
+                for (int i = grp * WPG; i < (grp + 1) * WPG; ++i)
+#pragma unroll
+                  for (int m = 0; m < 2; ++m) out[i][m][0][e] *= f, out[i][m][0][e + 2] *= f;
+              }
+            }
+            widest = 0.0f;
+#pragma unroll
+            for (int grp = 0; grp < NG; ++grp) {
+              scaled(grp);
+              widest = fmaxf(widest, sv[grp]);
+            }
+            __syncwarp();
+            if (lane == 0)
+#pragma unroll
+              for (int grp = 0; grp < NG; ++grp) s_unit[warp][grp] = unit[grp];
+          }
         }
         // Below 2^-60 a token counts as 2^-60, so that its probability and their sum stay in fp32's range.
         float lg = fmaxf(log2_approx(widest), -60.0f);
         if (!(lg < 1e9f)) lg = 0.0f;  // not finite: whoever sees the key becomes NaN
-        __syncwarp();                        // the previous tile's have been read
+        __syncwarp();                 // the previous tile's have been read
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
           // The offset part p (m + 8 s) is formed from the rounded weight x = p s as x (m / s + 8),
@@ -585,6 +645,9 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
           for (int k = 0; k < NG; ++k) bias[nt][k][e] += __shfl_xor_sync(~0u, bias[nt][k][e], o);
         }
+    float back[NG];  // from the groups' units
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) back[grp] = NG > 1 ? reciprocal_of_power(s_unit[warp][grp]) : 1.0f;
     const bool complete = u == w.item && ue == w.item + w.n_tiles;
     const int slot = ue == run_end;
     float* part = part_at(warp, slot);
@@ -600,10 +663,10 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           if (j < w.req.n) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-              const float b = bias[nt][i / WPG][e];
+              const float b = bias[nt][i / WPG][e], f = inv * back[i / WPG];
               uint2 v;
-              v.x = Elem<T>::from_f2((out[i][0][nt][e] + b) * inv, (out[i][0][nt][e + 2] + b) * inv);
-              v.y = Elem<T>::from_f2((out[i][1][nt][e] + b) * inv, (out[i][1][nt][e + 2] + b) * inv);
+              v.x = Elem<T>::from_f2((out[i][0][nt][e] + b) * f, (out[i][0][nt][e + 2] + b) * f);
+              v.y = Elem<T>::from_f2((out[i][1][nt][e] + b) * f, (out[i][1][nt][e + 2] + b) * f);
               *reinterpret_cast<uint2*>(o + 32 * i) = v;
             }
           }
@@ -614,9 +677,10 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           }
 #pragma unroll
           for (int i = 0; i < NW; ++i) {
-            const float b = bias[nt][i / WPG][e];
-            *reinterpret_cast<float4*>(part + col * (D + 4) + 32 * i + 4 * g) = make_float4(
-                out[i][0][nt][e] + b, out[i][0][nt][e + 2] + b, out[i][1][nt][e] + b, out[i][1][nt][e + 2] + b);
+            const float b = bias[nt][i / WPG][e], f = back[i / WPG];
+            *reinterpret_cast<float4*>(part + col * (D + 4) + 32 * i + 4 * g) =
+                make_float4((out[i][0][nt][e] + b) * f, (out[i][0][nt][e + 2] + b) * f, (out[i][1][nt][e] + b) * f,
+                            (out[i][1][nt][e + 2] + b) * f);
           }
         }
       }

@@ -176,3 +176,59 @@ def test_a_dominant_key_and_a_long_tail(D, group, dtype):
     err = (out.cpu().double() - want).abs()
     assert (err <= 8 * U[dtype] * torch.maximum(want.abs(), spread)).all()
     assert (err.flatten(1).norm(dim=1) <= 1.5 * U[dtype] * want.norm()).all(), err.norm(dim=(1, 2)).max() / want.norm()
+
+
+def group_factors(D, group, ratio, dtype):
+    """Per dim: one group in two `ratio` times the others, centred so that fp16 holds both."""
+    f = torch.ones(D // group)
+    f[1::2] = ratio
+    return (f / math.sqrt(ratio) if dtype == torch.float16 else f).repeat_interleave(group)
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("D,group", [(128, 64), (128, 32), (64, 32)])
+@pytest.mark.parametrize("ratio", [1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("total", [[1000, 33, 1], [100000]], ids=["short", "long"])
+def test_groups_of_different_size(total, ratio, D, group, dtype):
+    b = Batch(total, [1] * len(total), 4, 1, D, group, 64, dtype, seed=D + group)
+    b.v = (b.v.float() * group_factors(D, group, ratio, dtype)).to(dtype)
+    b.fill()
+    check_groups(b, group)
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("growing", [True, False])
+def test_groups_whose_size_changes_along_the_keys(growing, dtype):
+    """Values that grow or shrink by 1e4 along the keys, in one group of two, and single tokens
+    whose group is 100 times its neighbours'."""
+    T, D, group = 9000, 128, 32
+    b = Batch([T, 500], [1, 2], 8, 2, D, group, 32, dtype, seed=11)
+    n = b.v.shape[0]
+    size = torch.logspace(-2, 2, n)[:, None, None]
+    f = torch.ones(n, 1, D)
+    wide = (torch.arange(D) // group % 2 == 1)
+    f[:, :, wide] = size if growing else size.flip(0)
+    f[::1777, :, wide] *= 100
+    b.v = (b.v.float() * f).clamp(-60000, 60000).to(dtype)
+    b.fill()
+    check_groups(b, group)
+
+
+def test_parameters_of_hidden_tokens_do_not_matter():
+    """Tokens past the last key, beyond a query or before a window may hold any scale."""
+    D, group = 128, 32
+    for dtype in DT:
+        b = Batch([45, 300], [2, 1], 4, 1, D, group, 16, dtype, seed=12)
+        b.fill()
+        first = b.call(window=37)
+        big = 6e4 if dtype == torch.float16 else 1e30
+        params = b.cache.data[..., 16 * D:].view(dtype).unflatten(-1, (2, 16, D // group, 2))
+        flat = [s for s in range(b.cache.n_blocks * 16)]
+        held = set(b.slots)
+        for s in flat:   # every slot that no request holds, and those before the second one's window
+            if s not in held:
+                params[s // 16, 0, 0, :, s % 16] = big
+        for t in range(45, 45 + 300 - 37):
+            s = b.slots[t]
+            params[s // 16, 0, 0, :, s % 16] = big
+        assert torch.equal(b.call(window=37), first)
