@@ -447,7 +447,12 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         }
         // Below 2^-60 a token counts as 2^-60, so that its probability and their sum stay in fp32's range.
         float lg = fmaxf(log2_approx(widest), -60.0f);
-        if (!(lg < 1e9f)) lg = 0.0f;  // not finite: whoever sees the key becomes NaN
+        if (!(lg < 1e9f)) lg = 0.0f;
+        // A value row that is not finite makes its key's scores NaN, so that whoever sees the key becomes
+        // NaN, also where the weight would have been zero.
+        float bad = 0.0f;
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) bad = fmaf(0.0f, sv[grp], fmaf(0.0f, mv[grp], bad));
         __syncwarp();                 // the previous tile's have been read
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           unpack2<T>(wk[grp], sk, mk);
           pv[lane * NG + grp] =
               make_float4(sv[grp], small ? q : 0.0f, small ? 0.0f : fmaf(8.0f, sv[grp], mv[grp]), lg);
-          pk[lane * NG + grp] = make_float2(sk, mk);
+          pk[lane * NG + grp] = make_float2(grp ? sk : sk + bad, mk);
         }
         __syncwarp();
       }

@@ -232,3 +232,27 @@ def test_parameters_of_hidden_tokens_do_not_matter():
             s = b.slots[t]
             params[s // 16, 0, 0, :, s % 16] = big
         assert torch.equal(b.call(window=37), first)
+
+
+# ------------------------------------------------------------------ NaN, infinities, windows
+@pytest.mark.parametrize("key", [0, 100, 671, 672, 690, 699])
+@pytest.mark.parametrize("bound", [1, 100])
+def test_a_nan_value_of_no_weight_is_seen_wherever_a_tile_ends(key, bound):
+    """A NaN value whose weight underflows to zero makes a row that sees it NaN, in whole and in
+    partly hidden tiles of both kernels."""
+    b = Batch([700, 40], [1, 30], 2, 1, 64, 32, 16, torch.bfloat16, seed=6)
+    b.q = torch.ones_like(b.q)
+    b.k[key] = -40.0                # a score of -320
+    b.v[key, 0, 5] = math.nan
+    b.fill()
+    out = b.call(max_query_len=bound).cpu()
+    assert out[0].isnan().all() and not out[1:].isnan().any()
+
+
+def test_a_nan_value_outside_a_window_is_not_seen():
+    b = Batch([700, 40], [3, 30], 2, 1, 64, 64, 16, torch.bfloat16, seed=6)
+    b.v[600, 0, 5] = math.nan       # the last position that sees it with a window of 99 is 698
+    b.fill()
+    for bound in (1, 100):
+        out = b.call(window=99, max_query_len=bound).cpu()
+        assert out[:2].isnan().all() and not out[2:].isnan().any()
