@@ -10,12 +10,13 @@
 // cost one shift and four three-input logic operations.  For the keys the constants are taken back
 // by the value the accumulator starts with; for the values they are subtracted and the codes
 // centred, so that the sum over a long context does not cancel a large offset.  bf16 queries are
-// divided by a power of two per row.  p s is rounded to 16 bits for the product (the one rounding to
-// fewer than 32 bits besides the output); maxima, sums and outputs are fp32.  The reference exponent
-// holds the largest p s at 2^15, near the end of fp16's range, so that a weight keeps its eleven bits
-// down to 2^-29 of the largest and is dropped below 2^-40 of it (2^20 such weights are 2^-20 of it).
-// Where a head has several groups, s is in the group's own unit, so "the largest" is the group's own
-// up to what its scales differ from key to key.
+// divided by a power of two per row and group, exactly but for numbers 2^-14 below their group's
+// largest.  p s is rounded to 16 bits for the product (the one rounding to fewer than 32 bits besides
+// the output); maxima, sums and outputs are fp32.  The reference exponent holds the largest p s at
+// 2^15, near the end of fp16's range, so that a weight keeps its eleven bits down to 2^-29 of the
+// largest and is dropped below 2^-40 of it (2^20 such weights are 2^-20 of it).  Where a head has
+// several groups, s is in the group's own unit, so that "the largest" is the group's own up to what
+// its scales differ from key to key.
 //
 // Shape.  Both products are transposed (keys x queries and dims x queries, m16n8k16), so the
 // query heads that share a KV head fill the 8-wide side and 1 to 8 query rows cost the same.
@@ -282,11 +283,12 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     const int wt = w.tile_lo + (int)(u - w.item), we = wt + (int)(ue - u);
     const int pos0 = w.req.len - w.req.n, len = w.req.len;  // position of query 0
     // Queries: this lane's fragments (row g of each eight) in fp16, bf16 ones divided by the power
-    // of two of the row's largest, which is exact but for numbers 2^-14 below it.
+    // of two of the largest of their row and group, which is exact but for numbers 2^-14 below it.
+    constexpr int NU = Kv4Nib<T>::kFullRange ? NG : 1, WPU = NW / NU;
     uint32_t qf[NT][NW][4];
     float qs[NT][NG][2], qo[NT][NG][2];  // this lane's columns: sums of the queries, and minus the
                                          // sums weighted with the codes' offsets
-    float cf[NT][2];                     // score scale, in units of log2
+    float cf[NT][NU][2];                 // score scale, in units of log2, times the groups' powers of two
     int col_pos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -300,31 +302,34 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         if (j < w.req.n) v = *reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + c));
         qf[nt][i][0] = v.x, qf[nt][i][1] = v.y, qf[nt][i][2] = v.z, qf[nt][i][3] = v.w;
       }
-      float unit = 1.0f;
-      if (Kv4Nib<T>::kFullRange) {
-        float big = 0.0f;
+      float unit[NU];
 #pragma unroll
-        for (int i = 0; i < NW; ++i)
+      for (int u = 0; u < NU; ++u) {
+        unit[u] = 1.0f;
+        if (Kv4Nib<T>::kFullRange) {
+          float big = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float a, b;
-            unpack2<T>(qf[nt][i][e], a, b);
-            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
-          }
-        big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
-        // the power of two at or below `big`, within 2^+-120; an infinite or NaN row stays what it is
-        const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -120), 120);
-        unit = __uint_as_float((uint32_t)(127 + ex) << 23);
-        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+          for (int i = u * WPU; i < (u + 1) * WPU; ++i)
 #pragma unroll
-        for (int i = 0; i < NW; ++i)
+            for (int e = 0; e < 4; ++e) {
+              float a, b;
+              unpack2<T>(qf[nt][i][e], a, b);
+              big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+            }
+          big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+          big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
+          // the power of two at or below `big`, within 2^+-120; an infinite or NaN row stays what it is
+          const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -120), 120);
+          unit[u] = power_of_two(ex);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float a, b;
-            unpack2<T>(qf[nt][i][e], a, b);
-            qf[nt][i][e] = Elem<__half>::from_f2(a * inv, b * inv);
-          }
+          for (int i = u * WPU; i < (u + 1) * WPU; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float a, b;
+              unpack2<T>(qf[nt][i][e], a, b);
+              qf[nt][i][e] = Elem<__half>::from_f2(a * power_of_two(-ex), b * power_of_two(-ex));
+            }
+        }
       }
       float sum[NG] = {}, off[NG] = {};
 #pragma unroll
@@ -350,7 +355,8 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        cf[nt][e] = p.scale_log2 * __shfl_sync(~0u, unit, 8 * c + 4 * e);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) cf[nt][u][e] = p.scale_log2 * __shfl_sync(~0u, unit[u], 8 * c + 4 * e);
         col_pos[nt][e] = pos0 + (int)((uint32_t)(w.rb * ROWS + nt * 8 + 2 * c + e) / (uint32_t)p.G);
       }
     }
@@ -501,14 +507,11 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = (e < 2 ? ka.y : kb.y) * qs[nt][grp][e & 1];
-              s[m][nt][e] = fmaf(e < 2 ? ka.x : kb.x, acc[nt][e], grp ? s[m][nt][e] + v : v);
+              const float v = fmaf(e < 2 ? ka.x : kb.x, acc[nt][e], (e < 2 ? ka.y : kb.y) * qs[nt][grp][e & 1]);
+              const float f = cf[nt][grp * NU / NG][e & 1];
+              s[m][nt][e] = grp ? fmaf(v, f, s[m][nt][e]) : v * f;
             }
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][nt][e] *= cf[nt][e & 1];
       }
       const bool whole = tile >= full_lo && tile < full_hi;
       if (!whole) {

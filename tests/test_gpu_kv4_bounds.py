@@ -256,3 +256,16 @@ def test_a_nan_value_outside_a_window_is_not_seen():
     for bound in (1, 100):
         out = b.call(window=99, max_query_len=bound).cpu()
         assert out[:2].isnan().all() and not out[2:].isnan().any()
+
+
+@pytest.mark.parametrize("D,group", [(128, 64), (128, 32), (64, 32)])
+@pytest.mark.parametrize("ratio", [1e-4, 1e-6, 1e-8])
+def test_bf16_queries_whose_groups_differ(ratio, D, group):
+    """Queries that are small in the groups where the keys are large: each group's share of a score
+    is as large as any other's."""
+    b = Batch([1000, 33], [1, 1], 4, 1, D, group, 64, torch.bfloat16, seed=D + group)
+    f = group_factors(D, group, ratio, torch.bfloat16)
+    b.q = (b.q.float() * f).to(b.dtype)
+    b.k = (b.k.float() / f).to(b.dtype)
+    b.fill()
+    b.check()
