@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     // ---- a piece: tiles [u, ue) of item w
     const long long ue = min(run_end, w.item + w.n_tiles);
     const int wt = w.tile_lo + (int)(u - w.item), we = wt + (int)(ue - u);
-    const int pos0 = w.req.len - w.req.n, len = w.req.len;  // position of query 0
+    const int len = w.req.len;
     // Queries: this lane's fragments (row g of each eight) in fp16, bf16 ones divided by the power
     // of two of the largest of their row and group, which is exact but for numbers 2^-14 below it.
     constexpr int NU = Kv4Nib<T>::kFullRange ? NG : 1, WPU = NW / NU;
@@ -357,13 +357,13 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) cf[nt][u][e] = p.scale_log2 * __shfl_sync(~0u, unit[u], 8 * c + 4 * e);
-        col_pos[nt][e] = pos0 + (int)((uint32_t)(w.rb * ROWS + nt * 8 + 2 * c + e) / (uint32_t)p.G);
+        col_pos[nt][e] = kv4_position(w.req, (int)((uint32_t)(w.rb * ROWS + nt * 8 + 2 * c + e) / (uint32_t)p.G));
       }
     }
     // Tiles in [full_lo, full_hi) are visible to every row of the block.
     const int last_j = min((int)((uint32_t)(w.rb * ROWS + ROWS - 1) / (uint32_t)p.G), w.req.n - 1);
-    const int full_hi = max(0, pos0 + (int)((uint32_t)(w.rb * ROWS) / (uint32_t)p.G) + 1) / kTile;
-    const int full_lo = p.window > 0 ? (max(0, pos0 + last_j - p.window + 1) + kTile - 1) / kTile : 0;
+    const int full_hi = (kv4_position(w.req, (int)((uint32_t)(w.rb * ROWS) / (uint32_t)p.G)) + 1) / kTile;
+    const int full_lo = p.window > 0 ? (max(0, kv4_position(w.req, last_j) - p.window + 1) + kTile - 1) / kTile : 0;
 
     float out[NW][2][NT][4];
     float top[NT][2], sum[NT][2], bias[NT][NG][2];
@@ -415,11 +415,12 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         if constexpr (NG > 1) {
           if (__any_sync(~0u, widest > 1.0f)) {  // what was added up is brought to the new units
             const Work& x = s_item[warp];
-            const int t = tile * kTile + lane, first = x.req.len - x.req.n;
+            const int t = tile * kTile + lane;
             const int j0 = (int)((uint32_t)(x.rb * ROWS) / (uint32_t)p.G);
-            const int j1 = (int)((uint32_t)(x.rb * ROWS + ROWS - 1) / (uint32_t)p.G);
+            const int j1 = min((int)((uint32_t)(x.rb * ROWS + ROWS - 1) / (uint32_t)p.G), x.req.n - 1);
             // (what no row of the block sees may be anything)
-            const bool visible = t < x.req.len && t <= first + j1 && (p.window <= 0 || t > first + j0 - p.window);
+            const bool visible = t < x.req.len && t <= kv4_position(x.req, j1) &&
+                                 (p.window <= 0 || t > kv4_position(x.req, j0) - p.window);
 #pragma unroll
             for (int grp = 0; grp < NG; ++grp) {
               const float old = unit[grp];

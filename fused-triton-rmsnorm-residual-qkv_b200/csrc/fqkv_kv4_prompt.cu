@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       uint16_t* out = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + grow - j * p.G) * D;
       float ref = -INFINITY, sum = 0.0f;
       if (tile_used) {
-        const int pos = w.req.len - w.req.n + j;
+        const int pos = kv4_position(w.req, j);
         const int see_hi = live ? min(pos + 1, w.req.len) : w.req.len;      // keys [see_lo, see_hi)
         const int see_lo = live && p.window > 0 ? max(0, pos - p.window + 1) : 0;
         const bool warp_live = rows > t * 128 + (warp & 3) * 32;

@@ -36,6 +36,10 @@ __device__ __forceinline__ Kv4Request kv4_load_request(const Kv4AttnParams& p, i
   return q;
 }
 
+// Position of query j: -1 for those before the first token, which see nothing, so that a window of
+// any size can be taken off it.
+__device__ __forceinline__ int kv4_position(const Kv4Request& q, int j) { return max(-1, q.len - q.n + j); }
+
 // x * y / z for the cutting points: 32-bit arithmetic where the product allows it (a 64-bit
 // division costs about 0.3 us of a CTA's start).
 __device__ __forceinline__ long long kv4_muldiv(long long x, long long y, long long z, bool small) {
@@ -73,7 +77,7 @@ struct Kv4Work {
     const int j1 = min((int)((uint32_t)(rb * ROWS + ROWS - 1) / (uint32_t)p.G), q.n - 1);
     const int hi = max(0, min(q.len, q.len - q.n + j1 + 1));
     int lo = 0;
-    if (p.window > 0) lo = max(0, q.len - q.n + (int)((uint32_t)(rb * ROWS) / (uint32_t)p.G) - p.window + 1);
+    if (p.window > 0) lo = max(0, kv4_position(q, (int)((uint32_t)(rb * ROWS) / (uint32_t)p.G)) - p.window + 1);
     tile_lo = lo / TILE;
     n_tiles = max(1, (hi + TILE - 1) / TILE - tile_lo) + LEAD;
   }

@@ -269,3 +269,15 @@ def test_bf16_queries_whose_groups_differ(ratio, D, group):
     b.k = (b.k.float() / f).to(b.dtype)
     b.fill()
     b.check()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 40])
+@pytest.mark.parametrize("total,new", [(3, 6), (30, 60), (1, 40)])
+def test_largest_window_with_more_queries_than_tokens(total, new, window):
+    """Queries before the first token give zeros; the others see all that they do without a window."""
+    b = Batch([total, 50], [new, 9], 4, 1, 128, 128, 16, torch.bfloat16, seed=new)
+    b.fill()
+    for bound in (1, 100):
+        out = b.call(window=window, max_query_len=bound)
+        assert torch.equal(out, b.call(max_query_len=bound))
+        b.check(out)
