@@ -233,7 +233,11 @@ __device__ __forceinline__ void append_rows(const Kv4AppendParams& p, int head) 
     // The minimum is one of the 16-bit inputs, so it is stored exactly; the scale is rounded once,
     // and the codes are formed with the rounded scale that a reader multiplies them by.
     low[grp] = Elem<T>::to_f((uint16_t)lo);
-    const uint16_t scale16 = Elem<T>::from_f(__fmul_rn(Elem<T>::to_f((uint16_t)hi) - low[grp], 1.0f / 15.0f));
+    // At the end of the type's range the rounded scale may take code 15 past the largest number; one
+    // step lower does not, so that finite rows are read back finite by whoever rounds to 16 bits.
+    uint16_t scale16 = Elem<T>::from_f(__fmul_rn(Elem<T>::to_f((uint16_t)hi) - low[grp], 1.0f / 15.0f));
+    if (non_finite<T>(Elem<T>::from_f(__fmaf_rn(15.0f, Elem<T>::to_f(scale16), low[grp]))) && !non_finite<T>(scale16))
+      --scale16;
     scale[grp] = Elem<T>::to_f(scale16);
     bad |= non_finite<T>((uint16_t)lo) || non_finite<T>((uint16_t)hi) || non_finite<T>(scale16);
     param[grp] = (uint32_t)scale16 | (lo << 16);

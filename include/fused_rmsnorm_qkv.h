@@ -256,7 +256,9 @@ FQKV_API int fqkv_rope_split(const void* qkv, int64_t ldq, const void* cos, cons
  *   64 NG bytes     the keys' parameters: per token and group {scale, minimum}, 16-bit each
  *   64 NG bytes     the values' parameters, the same way
  * with D = head_dim and NG = D / group_size.  Code c of token t, dim d stands for
- *   scale[t, d / group_size] * c + minimum[t, d / group_size].
+ *   scale[t, d / group_size] * c + minimum[t, d / group_size],
+ * which must round to a finite number of the dtype for c = 15 where the parameters are finite (a
+ * cache that fqkv_kv4_append filled keeps that).
  * Byte places of the codes (low half of the byte for even j):
  *   keys    t * D/2 + c * D/8 + 4 i + 2 b + j / 2            d = 32 i + 8 c + 2 j + b
  *   values  16-bit word (h, g, c, i, b) for D = 128, (g, c, h, i, b) for D = 64, bits 4 j;
@@ -311,7 +313,8 @@ FQKV_API int fqkv_kv4_plan(const int32_t* context_lens, const int32_t* new_lens,
  *   slots [n_batch * n_seq]  distinct; negative: the token is skipped; past the cache: skipped
  *         and FQKV_STATUS_BAD_INDEX
  * Per token, head and group, in fp32: minimum = min x, scale = dtype((max x - min x) * (1/15)),
- * code = clamp(rint((x - minimum) / scale), 0, 15) (0 where scale is 0).  A head row with a
+ * code = clamp(rint((x - minimum) / scale), 0, 15) (0 where scale is 0).  Where 15 scale + minimum
+ * would round to infinity, the scale is the next smaller number.  A head row with a
  * NaN or an infinity (or a scale that overflows) is stored as NaN parameters.
  */
 FQKV_API int fqkv_kv4_append(const fqkv_kv4_cache* cache, const void* k, const void* v,

@@ -45,10 +45,13 @@ def plan(ctx, new, tables, free, n_free, block, n_tokens):
 
 def quantise(x: torch.Tensor, group: int):
     """(codes, scale, minimum) of rows (..., D): int codes, 16-bit scale and minimum (..., D / group).
-    A row with a NaN or an infinity, or whose scale overflows, has NaN parameters and codes 0."""
+    The scale is the next smaller number where 15 scale + minimum rounds to infinity.  A row with a
+    NaN or an infinity, or whose scale overflows, has NaN parameters and codes 0."""
     g = x.float().unflatten(-1, (-1, group))
     low = g.amin(-1)
     scale = ((g.amax(-1) - low) * torch.tensor(1 / 15, dtype=torch.float32)).to(x.dtype)
+    past = torch.isinf((15 * scale.double() + low.double()).float().to(x.dtype)) & torch.isfinite(scale)
+    scale = torch.where(past, (scale.view(torch.int16) - 1).view(x.dtype), scale)
     bad = (~torch.isfinite(x)).any(-1, keepdim=True) | (~torch.isfinite(scale)).any(-1, keepdim=True)
     s = scale.float()[..., None]
     code = torch.where(s > 0, torch.round((g - low[..., None]) / s), torch.zeros_like(g))

@@ -12,7 +12,7 @@ import torch
 
 from oracle import kv4 as ref
 from test_gpu_kv4 import DT, U, Batch, heads, i32
-from triton_fused_rmsnorm_qkv import device_status, kv4_append, kv4_attention, kv4_cache, kv4_plan
+from triton_fused_rmsnorm_qkv import device_status, kv4_append, kv4_attention, kv4_cache, kv4_gather, kv4_plan
 
 pytestmark = pytest.mark.gpu
 IDS = ["bf16", "fp16"]
@@ -281,3 +281,44 @@ def test_largest_window_with_more_queries_than_tokens(total, new, window):
         out = b.call(window=window, max_query_len=bound)
         assert torch.equal(out, b.call(max_query_len=bound))
         b.check(out)
+
+
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 32), (64, 64)])
+@pytest.mark.parametrize("low", [0.0, -65504.0])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_fp16_numbers_at_the_end_of_the_range(where, low, D, group):
+    """Values of up to 65504 whose scale is rounded up, so that 15 steps would end at 65520 or more:
+    rows that do not see the key are untouched and rows that see it are finite.  (Queries are small
+    where the key is large, so that its error of one part in 2048 moves no score by more than u.)"""
+    for total, new, bound in (([300, 50], [40, 1], None), ([300, 50], [2, 1], 1), ([290, 50], [200, 3], 500)):
+        b = Batch(total, new, 4, 1, D, group, 16, torch.float16, seed=D)
+        x = b.k if where == "k" else b.v
+        key = 299 if total[0] == 300 else 200
+        x[key, 0, ::2], x[key, 0, 1::2] = low, 65504.0
+        if where == "k":
+            b.q = b.q * 1e-5
+        b.fill()
+        b.check(max_query_len=bound)
+        b.check(max_query_len=bound, window=70)
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 32), (64, 64)])
+def test_finite_rows_are_read_back_finite(D, group, dtype):
+    """Rows between a low number and the type's largest: the stored bytes are the definition's, and
+    no number read back is infinite or further off than a step."""
+    top = torch.finfo(dtype).max
+    low = torch.linspace(-1, 1, 97) * top if dtype == torch.float16 else torch.linspace(-0.0039, 1, 97) * top
+    x = torch.full((97, 1, D), top).to(dtype)
+    x[:, 0, ::2] = low.to(dtype)[:, None]
+    x[:, 0, 1::8] = (top * 0.9 + low * 0.1).to(dtype)[:, None]
+    cache = kv4_cache(7, 1, D, block_size=16, group_size=group, dtype=dtype)
+    slots = i32(list(range(97)))
+    kv4_append(cache, x.cuda(), x.cuda(), slots)
+    code, scale, low16 = ref.quantise(x, group)
+    assert torch.isfinite(scale).all()
+    want = ref.values(code, scale, low16).float().to(dtype)
+    for got in kv4_gather(cache, slots):
+        assert torch.isfinite(got).all() and torch.equal(got.cpu(), want)
+        step = scale.double().repeat_interleave(group, -1)
+        assert ((got.cpu().double() - x.double()).abs() <= step).all()
