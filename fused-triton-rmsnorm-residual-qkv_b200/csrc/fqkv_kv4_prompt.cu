@@ -3,8 +3,8 @@
 //
 // Mathematics.  S = Q K^T and O = P V with the online softmax: P = exp2(c S - c ref), where c is
 // the score scale times log2(e) and ref a row maximum that is only moved (and O and the row sum
-// rescaled) when the true maximum exceeds it by 8 in the exponent; P stays below 2^8 and the
-// quotient O / sum does not depend on ref.  Keys and values are formed once per CTA as
+// rescaled) when the true maximum exceeds it by 8 in the exponent; P stays below 2^8 (in bf16, whose
+// values may be as large as fp32's, below 2^-16) and the quotient O / sum does not depend on ref.  Keys and values are formed once per CTA as
 // round16(scale * code + minimum), one rounding to the cache's type (the operand type of the
 // product); P is rounded to the same type, row sums, maxima and accumulators are fp32.
 //
@@ -42,6 +42,8 @@ constexpr int kPMinTiles = 4;
 // What beginning and ending an item costs, in steps (measured on a prompt of 4096 tokens, whose
 // CTAs have between 2 and 14 items: 291, 247, 220, 201 us with 0, 1, 2, 3).
 constexpr int kPLead = 3;
+// P is held this many powers of two lower in bf16: 2^16 products with the largest number fit O.
+constexpr float kPLower = 24.0f;
 using Work = Kv4Work<kPRows, kPTile, kPThreads, 1, kPLead>;
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16.
@@ -293,7 +295,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
                 }
               }
               // A NaN or an infinite score makes the whole row NaN.
-              const float off = top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : -ref * c;
+              const float off =
+                  top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : fmaf(-ref, c, kBf16 ? -kPLower : 0.0f);
               const uint64_t off2 = pack2(off, off);
               exp32<T>(s, c2, off2, at, sum2);  // P (16-bit pairs) over the half's first 32 columns
               exp32<T>(s + 32, c2, off2, at + 16, sum2);

@@ -322,3 +322,15 @@ def test_finite_rows_are_read_back_finite(D, group, dtype):
         assert torch.isfinite(got).all() and torch.equal(got.cpu(), want)
         step = scale.double().repeat_interleave(group, -1)
         assert ((got.cpu().double() - x.double()).abs() <= step).all()
+
+
+def test_bf16_numbers_at_the_end_of_the_range():
+    """As above in bf16, -1.3e36 .. 3.39e38; the product with a probability stays in range."""
+    top = torch.finfo(torch.bfloat16).max
+    b = Batch([300], [40], 4, 1, 128, 128, 16, torch.bfloat16, seed=4)
+    b.v[280, 0, ::2], b.v[280, 0, 1::2] = -1.3e36, top
+    b.fill()
+    out = b.call().cpu()
+    want, _ = b.reference()
+    assert torch.isfinite(out).all()
+    assert (out[:20].double() - want[:20]).norm() <= 1.5 * U[torch.bfloat16] * want[:20].norm()
