@@ -69,6 +69,7 @@ struct Kv4AttnParams {
   int64_t o_t;
   int* counters;
   float* partial;
+  int withhold;                   // FQKV_FLAG_TEST_WITHHOLD: one arrival of CTA 0 is left out
 };
 
 cudaError_t launch_kv4_plan(const Kv4PlanParams& p, bool pdl, cudaStream_t stream);

@@ -39,8 +39,10 @@ int check_cache(const fqkv_kv4_cache* c, Kv4Cache* out) {
   return 0;
 }
 
-int check_flags(int64_t flags) {
-  return flags & ~(int64_t)FQKV_FLAG_PDL ? api_fail(FQKV_ERR_SCHEDULE, "the cache's calls take FQKV_FLAG_PDL only") : 0;
+int check_flags(int64_t flags, int64_t also = 0) {
+  return flags & ~(FQKV_FLAG_PDL | also)
+             ? api_fail(FQKV_ERR_SCHEDULE, "the cache's calls take FQKV_FLAG_PDL (attention: FQKV_FLAG_TEST_WITHHOLD)")
+             : 0;
 }
 
 int done(cudaError_t e, const char* what) { return e == cudaSuccess ? 0 : api_cuda_fail(e, what); }
@@ -97,8 +99,8 @@ extern "C" FQKV_API int fqkv_kv4_plan(const int32_t* context_lens, const int32_t
       return api_fail(FQKV_ERR_ALIAS, "block_tables, which the plan writes, overlaps another argument");
     for (int j = i < 6 ? i + 1 : 10; j < 10; ++j)
       if (overlap(words[i], words[j]))
-        return api_fail(FQKV_ERR_ALIAS, "an output of the plan overlaps an input or another output: every CTA reads all "
-                                        "lengths, the free list and n_free");
+        return api_fail(FQKV_ERR_ALIAS, "an output of the plan overlaps an input or another output: every CTA reads "
+                                        "all lengths, the free list and n_free");
   }
   if (int rc = check_flags(flags)) return rc;
   int sms = 0;
@@ -191,7 +193,7 @@ extern "C" FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const vo
   const int64_t need = fqkv_kv4_workspace_bytes(n_q_heads, c.n_kv, c.D, max_query_len);
   if (!workspace || workspace_bytes < need) return api_fail(FQKV_ERR_WORKSPACE, "workspace missing or too small");
   if (!aligned(workspace, 256)) return api_fail(FQKV_ERR_ALIGN, "the workspace must be 256-byte aligned");
-  if (int rc = check_flags(flags)) return rc;
+  if (int rc = check_flags(flags, FQKV_FLAG_TEST_WITHHOLD)) return rc;
   int sms = 0;
   if (int rc = api_sm100(&sms)) return rc;
   Kv4AttnParams p{};
@@ -208,6 +210,7 @@ extern "C" FQKV_API int fqkv_kv4_attention(const fqkv_kv4_cache* cache, const vo
   p.out = static_cast<uint16_t*>(out), p.o_t = out_stride_t;
   p.counters = static_cast<int*>(workspace);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv4CounterBytes);
+  p.withhold = (flags & FQKV_FLAG_TEST_WITHHOLD) != 0;
   const bool pdl = flags & FQKV_FLAG_PDL, bf16 = cache->dtype == FQKV_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return done(for_prompts(p.G, max_query_len) ? launch_kv4_attn_prompt(p, sms, bf16, pdl, st)

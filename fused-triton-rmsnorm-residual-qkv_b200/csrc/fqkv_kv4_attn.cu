@@ -102,7 +102,9 @@ __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& lo, fl
 
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-__device__ __forceinline__ float reciprocal_of_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+__device__ __forceinline__ float reciprocal_of_power(float x) {
+  return __uint_as_float((254u << 23) - __float_as_uint(x));
+}
 
 // a / b by an approximate reciprocal and one step of refinement; exact where the quotient is a
 // small integer.  Not meaningful for b = 0 or subnormal.
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     src = address(2 * ahead_tile + lane);
     src_next = 2 * ahead_end > 2 * ahead_tile + 32 ? address(2 * ahead_tile + 32 + lane) : nullptr;
   };
-  const auto copy_next = [&]() {
+  const auto copy_next = [&](bool withhold) {
     if (to_copy <= 0) return;
     if (ahead_tile == ahead_end) {
       Work x = s_ahead[warp];
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       if (ahead_end > src_tile + 16) src_next = address(2 * (src_tile + 16) + lane);
     }
     const uint32_t k = (uint32_t)(lane - 2 * (ahead_tile - src_tile));
-    if (k < 2) {  // the lanes of this tile's records; past the last record there is nothing to wait for
+    if (k < 2 && !withhold) {  // the lanes of this tile's records; past the last record there is nothing to wait for
       if (src) {
         mbar_arrive_expect_tx(&s_bar[warp][stage_in], REC);
         bulk_load(smem_u32(ring + (stage_in * 2 + k) * REC), src, REC, &s_bar[warp][stage_in]);
@@ -273,10 +275,11 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
   };
   if (to_copy > 0) enter();
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) copy_next();
+  for (int s = 0; s < kStages; ++s) copy_next(s == 0 && p.withhold && blockIdx.x == 0 && warp == 0);
 
   int stage = 0;
   uint32_t parity = 0;  // bit s: phase of ring stage s
+  bool ok = true;       // after a wait that ran out nothing is copied or waited for, and rows become NaN
   for (long long u = w.a; u < run_end;) {
     // ---- a piece: tiles [u, ue) of item w
     const long long ue = min(run_end, w.item + w.n_tiles);
@@ -389,8 +392,19 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       if (lane < NG) s_unit[warp][lane] = power_of_two(kMostUnit);
       __syncwarp();
     }
-    for (int tile = wt; tile < we; ++tile) {
-      mbar_wait(&s_bar[warp][stage], (parity >> stage) & 1u);
+    for (int tile = ok ? wt : we; tile < we; ++tile) {
+      if (!__all_sync(~0u, mbar_wait(&s_bar[warp][stage], (parity >> stage) & 1u))) {
+        // Nothing may be in flight into the ring when it is used for parts and when the block ends.
+        int at = stage;
+        do {
+          mbar_wait(&s_bar[warp][at], (parity >> at) & 1u);
+          at = at + 1 == kStages ? 0 : at + 1;
+        } while (at != stage_in);
+        __syncwarp();
+        to_copy = 0;
+        ok = false;
+        break;
+      }
       parity ^= 1u << stage;
       const uint8_t* rec = ring + stage * 2 * REC;
       // ---- parameters: each lane prepares one token's
@@ -427,7 +441,8 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
               unit[grp] = 1.0f;
               scaled(grp);
               // (positive floats are ordered as integers)
-              const uint32_t most = __reduce_max_sync(~0u, visible && sv[grp] < INFINITY ? __float_as_uint(sv[grp]) : 0u);
+              const bool counts = visible && sv[grp] < INFINITY;
+              const uint32_t most = __reduce_max_sync(~0u, counts ? __float_as_uint(sv[grp]) : 0u);
               const int up = max(-kMostUnit, min(kMostUnit, 126 - kUnitRoom - (int)(most >> 23)));
               unit[grp] = fminf(old, power_of_two(up));
               const float f = unit[grp] * reciprocal_of_power(old);
@@ -639,10 +654,14 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         }
       }
       __syncwarp();  // every lane has read this stage
-      copy_next();
+      copy_next(false);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
+    if (!ok) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = NAN;
+    }
     // ---- the piece's sums over the keys
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -699,10 +718,9 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     if (u < run_end) {
       Work x = w;
       __syncwarp();
-      const bool more = x.next(p);
+      x.next(p);  // (where lengths changed under the kernel and none is left, the tiles copied are still consumed)
       if (lane == 0) s_item[warp] = x;
       __syncwarp();
-      if (!more) break;
     }
   }
 

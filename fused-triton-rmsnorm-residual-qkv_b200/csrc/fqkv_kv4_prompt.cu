@@ -4,9 +4,10 @@
 // Mathematics.  S = Q K^T and O = P V with the online softmax: P = exp2(c S - c ref), where c is
 // the score scale times log2(e) and ref a row maximum that is only moved (and O and the row sum
 // rescaled) when the true maximum exceeds it by 8 in the exponent; P stays below 2^8 (in bf16, whose
-// values may be as large as fp32's, below 2^-16) and the quotient O / sum does not depend on ref.  Keys and values are formed once per CTA as
-// round16(scale * code + minimum), one rounding to the cache's type (the operand type of the
-// product); P is rounded to the same type, row sums, maxima and accumulators are fp32.
+// values may be as large as fp32's, below 2^-16) and the quotient O / sum does not depend on ref.
+// Keys and values are formed once per CTA as round16(scale * code + minimum), one rounding to the
+// cache's type (the operand type of the product); P is rounded to the same type, row sums, maxima
+// and accumulators are fp32.
 //
 // Shape.  A CTA takes 256 query rows of one KV head (all heads that share it, so the keys are
 // unpacked once for them) as two tiles of 128 and walks the keys 128 at a time:
@@ -157,6 +158,7 @@ struct Bars {
   uint64_t q_full;                  // the queries of an item
   uint64_t s_full[2][2], p_full[2][2];  // [tile][half]: scores formed; probabilities written
   uint64_t o_done[2][2];                // [tile][half]: an item's last step added to O
+  uint64_t drained;                     // every product that was issued has completed
 };
 
 // Whether a scale or a minimum (packed pair) is a NaN or an infinity.
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       }
     }
     mbar_init(&bars.q_full, 4);
+    mbar_init(&bars.drained, 1);
     fence_mbarrier_init_cluster();
   }
   pdl_wait();
@@ -295,8 +298,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
                 }
               }
               // A NaN or an infinite score makes the whole row NaN.
-              const float off =
-                  top != top || ref == INFINITY ? NAN : ref == -INFINITY ? 0.0f : fmaf(-ref, c, kBf16 ? -kPLower : 0.0f);
+              const float off = top != top || ref == INFINITY ? NAN
+                                : ref == -INFINITY            ? 0.0f
+                                                              : fmaf(-ref, c, kBf16 ? -kPLower : 0.0f);
               const uint64_t off2 = pack2(off, off);
               exp32<T>(s, c2, off2, at, sum2);  // P (16-bit pairs) over the half's first 32 columns
               exp32<T>(s + 32, c2, off2, at + 16, sum2);
@@ -324,6 +328,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         wait(&bars.o_done[t][1], o_phase);
         o_phase ^= 1u;
         tc_fence_after();
+        if (!ok) sum = NAN;
       }
       if (complete) {
         if (tile_used) {
@@ -438,7 +443,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
     const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale negates the keys
     const uint32_t magic = kv4_opaque(Kv4Nib<T>::kOffset2, p.n_q);
     uint32_t it = 0;
-    bool ok = true;
+    bool ok = true;  // the same in all lanes, which meet at every tile
+    const auto wait = [&](uint64_t* bar, uint32_t phase) { ok = __all_sync(~0u, ok && mbar_wait(bar, phase & 1u)); };
     uint32_t kc[4 * NW], kp[NG], vq[NG], vc[4 * NW], vp[8 * NG];
     for (long long u = w.u0; u < w.u1 && ok;) {
       const long long ue = min(w.u1, w.item + w.n_tiles);
@@ -532,7 +538,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       // The item's queries, once the previous item's last scores have been formed.
       const auto copy_q = [&]() {
         constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row; rows copied at a time
-        if (it > 0) ok = ok && mbar_wait(&bars.k_empty[(it - 1) & 1], ((it - 1) >> 1) & 1u);
+        if (it > 0) wait(&bars.k_empty[(it - 1) & 1], (it - 1) >> 1);
         const int ch = key % CH, dj = STEP / p.G, dh = STEP % p.G;
         int row = key / CH, j = (int)((uint32_t)(w.rb * kPRows + row) / (uint32_t)p.G);
         int h = w.rb * kPRows + row - j * p.G;
@@ -553,7 +559,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
         const uint32_t phase = (it >> 1) & 1u;
         uint8_t* k_tile = smem + (2 + stage) * OP;
         uint8_t* v_tile = smem + (4 + stage) * OP;
-        if (it >= 2) ok = ok && mbar_wait(&bars.k_empty[stage], phase ^ 1u);
+        if (it >= 2) wait(&bars.k_empty[stage], phase ^ 1u);
         // ---- keys: a word is eight dims, one 16-byte chunk of the key's row
         uint32_t hide = flip;  // a key whose value row is NaN scores NaN, so whoever sees it becomes NaN
 #pragma unroll
@@ -577,7 +583,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           }
         }
         fence_proxy_async_smem();
-        warp_arrive(&bars.k_full[stage]);
+        if (!(p.withhold && it == 0 && dw == 0 && blockIdx.x == 0)) warp_arrive(&bars.k_full[stage]);
         if (tile == first) copy_q();
         if (tile + 1 < last) {
           advance();
@@ -588,7 +594,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
           fence_proxy_async_smem();
           warp_arrive(&bars.q_full);
         }
-        if (it >= 2) ok = ok && mbar_wait(&bars.v_empty[stage], phase ^ 1u);
+        if (it >= 2) wait(&bars.v_empty[stage], phase ^ 1u);
         // ---- values: rows are dims, a chunk is eight tokens
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -666,6 +672,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       wait(&bars.k_full[it & 1], it >> 1);
       wait(&bars.q_full, q_phase);
       q_phase ^= 1u;
+      if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
@@ -688,7 +695,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
             if (t < tiles) {
               wait(&bars.p_full[t][h], p_phase[t]);
               tc_fence_after();
-              if (elect_one()) {
+              if (ok && elect_one()) {
                 issue_o(t, h, it, x > 0 || h > 0);
                 if (ahead) issue_s(t, h, it + 1);
                 else umma_commit(&bars.o_done[t][h]);
@@ -705,8 +712,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4AttnP
       u = ue;
       if (u >= w.u1 || !w.next(p)) break;
     }
+    // No product may be in flight when TMEM is freed and the block ends, also after a wait that ran out.
+    if (elect_one()) umma_commit(&bars.drained);
+    __syncwarp();
+    mbar_wait(&bars.drained, 0);
   }
-  // Every product has completed: each tile's last O was waited for, and its scores come before it.
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -80,7 +80,9 @@ extern "C" {
                                        fqkv_test_set_wait_limit_ns), FQKV_STATUS_WAIT_TIMEOUT is
                                        recorded and the kernel winds down and returns.  `out`
                                        is undefined after such a launch; residual_out is
-                                       written as usual. */
+                                       written as usual.  fqkv_kv4_attention takes it too: one
+                                       arrival of its first CTA is left out, and rows that
+                                       needed it are NaN */
 
 /* Error codes (> 0). */
 #define FQKV_ERR_NULL        1  /* a required pointer is NULL                                */

@@ -12,7 +12,7 @@ import torch
 
 from oracle import kv4 as ref
 from test_gpu_kv4 import DT, U, Batch, heads, i32
-from triton_fused_rmsnorm_qkv import device_status, kv4_append, kv4_attention, kv4_cache, kv4_gather, kv4_plan
+from triton_fused_rmsnorm_qkv import _lib, device_status, kv4_append, kv4_attention, kv4_cache, kv4_gather, kv4_plan
 
 pytestmark = pytest.mark.gpu
 IDS = ["bf16", "fp16"]
@@ -72,8 +72,8 @@ def test_a_padded_step_of_a_plan():
     n_kv, D, block, T = 2, 64, 16, 24
     cache = kv4_cache(8, n_kv, D, block_size=block)
     tables = torch.full((2, 4), -1, dtype=torch.int32, device="cuda")
-    plan = kv4_plan(i32([0, 0]), i32([5, 9]), tables, torch.randperm(8, device="cuda").int(), i32([8]), block_size=block,
-                    n_tokens=T)
+    free = torch.randperm(8, device="cuda").int()
+    plan = kv4_plan(i32([0, 0]), i32([5, 9]), tables, free, i32([8]), block_size=block, n_tokens=T)
     k, v, q = (heads(s, T, h, D) for s, h in ((1, n_kv), (2, n_kv), (3, 8)))
     kv4_append(cache, k.cuda(), v.cuda(), plan.slots)
     out = torch.full((T, 8, D), math.nan, dtype=q.dtype, device="cuda")
@@ -334,3 +334,39 @@ def test_bf16_numbers_at_the_end_of_the_range():
     want, _ = b.reference()
     assert torch.isfinite(out).all()
     assert (out[:20].double() - want[:20]).norm() <= 1.5 * U[torch.bfloat16] * want[:20].norm()
+
+
+# ------------------------------------------------------------------ a wait that runs out
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 32), (64, 64)])
+@pytest.mark.parametrize("total,new,bound", [([3000, 40], [1, 1], 1), ([900, 40], [130, 9], 130)],
+                         ids=["split", "prompt"])
+def test_a_withheld_arrival_times_out_and_the_next_launch_is_clean(total, new, bound, D, group):
+    """One arrival on one barrier is left out (FQKV_FLAG_TEST_WITHHOLD) and the limit is 1 ms: the
+    launch returns, the status reports it, rows are right or NaN, the arrival counters are zero
+    and the next launch is as if nothing had been."""
+    b = Batch(total, new, 8, 2, D, group, 16, torch.bfloat16, seed=13)
+    b.fill()
+    first = b.call(max_query_len=bound)
+    b.check(first)
+    q, tables, lens, start = b.q.cuda(), i32(b.tables), i32(b.total), i32(b.start)
+    out = torch.zeros_like(first)
+    need = _lib.load().fqkv_kv4_workspace_bytes(8, 2, D, bound)
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    args = [b.cache._ptr, q.data_ptr(), q.stride(0), q.stride(0), q.stride(1), 8, start.data_ptr(), q.shape[0], 0,
+            len(total), bound, tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr(), 0, D ** -0.5,
+            out.data_ptr(), out.stride(0), ws.data_ptr(), need]
+    stream = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    _lib.set_wait_limit_ns(1_000_000)
+    try:
+        assert _lib.kv4["attention"](*args, _lib.FLAG_PDL | _lib.FLAG_TEST_WITHHOLD, stream) == 0, _lib.last_error()
+        torch.cuda.synchronize()
+        status = device_status()
+    finally:
+        _lib.set_wait_limit_ns(0)
+    assert status == _lib.STATUS_WAIT_TIMEOUT
+    missing = out.isnan()
+    assert missing.any() and torch.equal(out[~missing], first[~missing])
+    assert int(ws[:4096].count_nonzero()) == 0
+    assert _lib.kv4["attention"](*args, _lib.FLAG_PDL, stream) == 0
+    assert torch.equal(out, first)
