@@ -138,10 +138,12 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
 // its accumulators only at twelve warps an SM: 54 us against 44 us for two items of eight (16
 // requests of 500 to 6000 tokens, 16 rows on 8 KV heads), 84 against 62 us at 24 rows.
 constexpr int NT = 1;
-// Warps of a CTA, two CTAs on an SM; fewer where eight rings of larger records leave no room.
+// Warps of a CTA, two CTAs on an SM; fewer where eight rings of larger records leave no room (seven
+// of two groups fit, but have 128 registers a thread, as eight have, which spill: 64 requests with
+// groups of 64 take 117.7 us with seven and 113.5 with six).
 template <int D, int NG>
 constexpr int warps() {
-  return D == 128 ? (NG == 4 ? 6 : NG == 2 ? 7 : 8) : 8;
+  return D == 128 ? (NG == 1 ? 8 : 6) : 8;
 }
 // Ring stages of a warp, about 9 KB.
 template <int D>
