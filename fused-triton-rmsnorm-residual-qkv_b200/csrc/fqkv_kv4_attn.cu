@@ -161,7 +161,7 @@ constexpr int part_floats() {
   return 8 * NT * (D + 4);
 }
 // A stage's parameters as the lanes use them, per token and group: the values' {s, r, z, log2 of
-// the token's largest s}, s and z in the group's unit, then the keys' {s, m}.
+// the token's largest s less kRoom}, s and z in the group's unit, then the keys' {s, m}.
 template <int NG>
 constexpr int param_bytes() {
   return kTile * NG * 24;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           }
         }
         // Below 2^-60 a token counts as 2^-60, so that its probability and their sum stay in fp32's range.
-        float lg = fmaxf(log2_approx(widest), -60.0f);
+        float lg = fmaxf(log2_approx(widest), -60.0f) - kRoom;
         if (!(lg < 1e9f)) lg = 0.0f;
         // A value row that is not finite makes its key's scores NaN, so that whoever sees the key becomes
         // NaN, also where the weight would have been zero.
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e] - kRoom;
+        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];
       // ---- probabilities, and the products with the values
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
