@@ -416,16 +416,16 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         lds_words<NG>(at, wk);
         lds_words<NG>(at + 64 * NG, wv);
         float sv[NG], mv[NG], unit[NG], widest = 0.0f;
-        const auto scaled = [&](int grp) {
+        const auto scaled = [&](int grp, float u) {
           unpack2<T>(wv[grp], sv[grp], mv[grp]);
           // A scale of zero goes with codes of zero; any scale then stands for the same numbers.
           if (sv[grp] == 0.0f) sv[grp] = fmaxf(fabsf(mv[grp]), 1e-20f);
-          if (NG > 1) sv[grp] *= unit[grp], mv[grp] *= unit[grp];
+          if (NG > 1) sv[grp] *= u, mv[grp] *= u;
         };
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
           unit[grp] = NG > 1 ? s_unit[warp][grp] : 1.0f;
-          scaled(grp);
+          scaled(grp, unit[grp]);
           widest = fmaxf(widest, sv[grp]);
         }
         if constexpr (NG > 1) {
@@ -440,8 +440,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
             for (int grp = 0; grp < NG; ++grp) {
               const float old = unit[grp];
-              unit[grp] = 1.0f;
-              scaled(grp);
+              scaled(grp, 1.0f);
               // (positive floats are ordered as integers)
               const bool counts = visible && sv[grp] < INFINITY;
               const uint32_t most = __reduce_max_sync(~0u, counts ? __float_as_uint(sv[grp]) : 0u);
@@ -460,7 +459,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
             widest = 0.0f;
 #pragma unroll
             for (int grp = 0; grp < NG; ++grp) {
-              scaled(grp);
+              scaled(grp, unit[grp]);
               widest = fmaxf(widest, sv[grp]);
             }
             __syncwarp();

@@ -170,7 +170,7 @@ struct Kv4Work {
       }
       if (!one) __syncthreads();
     }
-    if (p.query_start) {
+    if (__builtin_expect(s.rows[0] > 0 || s.rows[1] < p.T, 0)) {
       zero_rows(p, 0, s.rows[0]);
       zero_rows(p, s.rows[1], p.T);
     }
