@@ -134,10 +134,10 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// Eights of query rows of an item.  Sixteen rows unpack the codes half as often, but leave a warp
+// Query rows of an item.  Sixteen rows unpack the codes half as often, but leave a warp
 // its accumulators only at twelve warps an SM: 54 us against 44 us for two items of eight (16
 // requests of 500 to 6000 tokens, 16 rows on 8 KV heads), 84 against 62 us at 24 rows.
-constexpr int NT = 1;
+constexpr int kRows = 8;
 // Warps of a CTA, two CTAs on an SM; fewer where eight rings of larger records leave no room (seven
 // of two groups fit, but have 128 registers a thread, as eight have, which spill: 64 requests with
 // groups of 64 take 117.7 us with seven and 113.5 with six).
@@ -158,7 +158,7 @@ constexpr int ring_bytes() {
 // float4 stores of a quarter-warp (four columns, two dim groups) meet eight different bank groups.
 template <int D>
 constexpr int part_floats() {
-  return 8 * NT * (D + 4);
+  return kRows * (D + 4);
 }
 // A stage's parameters as the lanes use them, per token and group: the values' {s, r, z, log2 of
 // the token's largest s less kRoom}, s and z in the group's unit, then the keys' {s, m}.
@@ -181,7 +181,7 @@ template <typename T, int D, int NG>
 __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     kv4_attn_split_kernel(const Kv4AttnParams p) {
   constexpr int WARPS = warps<D, NG>(), THREADS = WARPS * 32;
-  constexpr int ROWS = 8 * NT;           // query rows of an item
+  constexpr int ROWS = kRows;            // query rows of an item
   constexpr int REC = kv4_record_bytes(D, NG), kStages = stages<D>();
   constexpr int NW = D / 32;             // 32-dim blocks: words per lane and key row
   constexpr int WPG = NW / NG;           // words of one scale group
@@ -287,17 +287,16 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     const long long ue = min(run_end, w.item + w.n_tiles);
     const int wt = w.tile_lo + (int)(u - w.item), we = wt + (int)(ue - u);
     const int len = w.req.len;
-    // Queries: this lane's fragments (row g of each eight) in fp16, bf16 ones divided by the power
-    // of two of the largest of their row and group, which is exact but for numbers 2^-14 below it.
+    // Queries: this lane's fragments (row g) in fp16, bf16 ones divided by the power of two of the
+    // largest of their row and group, which is exact but for numbers 2^-14 below it.
     constexpr int NU = Kv4Nib<T>::kFullRange ? NG : 1, WPU = NW / NU;
-    uint32_t qf[NT][NW][4];
-    float qs[NT][NG][2], qo[NT][NG][2];  // this lane's columns: sums of the queries, and minus the
-                                         // sums weighted with the codes' offsets
-    float cf[NT][NU][2];                 // score scale, in units of log2, times the groups' powers of two
-    int col_pos[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = w.rb * ROWS + nt * 8 + g;
+    uint32_t qf[NW][4];
+    float qs[NG][2], qo[NG][2];  // this lane's columns: sums of the queries, and minus the sums
+                                 // weighted with the codes' offsets
+    float cf[NU][2];             // score scale, in units of log2, times the groups' powers of two
+    int col_pos[2];
+    {
+      const int row = w.rb * ROWS + g;
       const int j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
       const uint16_t* qrow = p.q + (p.query_start ? (int64_t)(w.req.start + j) * p.q_t : w.r * p.q_r + j * p.q_t) +
                              (int64_t)(w.kvh * p.G + h) * p.q_h;
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       for (int i = 0; i < NW; ++i) {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (j < w.req.n) v = *reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + c));
-        qf[nt][i][0] = v.x, qf[nt][i][1] = v.y, qf[nt][i][2] = v.z, qf[nt][i][3] = v.w;
+        qf[i][0] = v.x, qf[i][1] = v.y, qf[i][2] = v.z, qf[i][3] = v.w;
       }
       float unit[NU];
 #pragma unroll
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float a, b;
-              unpack2<T>(qf[nt][i][e], a, b);
+              unpack2<T>(qf[i][e], a, b);
               big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
             }
           big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
@@ -331,8 +330,8 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float a, b;
-              unpack2<T>(qf[nt][i][e], a, b);
-              qf[nt][i][e] = Elem<__half>::from_f2(a * power_of_two(-ex), b * power_of_two(-ex));
+              unpack2<T>(qf[i][e], a, b);
+              qf[i][e] = Elem<__half>::from_f2(a * power_of_two(-ex), b * power_of_two(-ex));
             }
         }
       }
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float a, b;
-          unpack2<__half>(qf[nt][i][e], a, b);
+          unpack2<__half>(qf[i][e], a, b);
           sum[i / WPG] += a + b;
           off[i / WPG] -= (e & 1 ? 64.0f : 1024.0f) * (a + b);
         }
@@ -354,15 +353,15 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         off[k] += __shfl_xor_sync(~0u, off[k], 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          qs[nt][k][e] = __shfl_sync(~0u, sum[k], 8 * c + 4 * e);
-          qo[nt][k][e] = __shfl_sync(~0u, off[k], 8 * c + 4 * e);
+          qs[k][e] = __shfl_sync(~0u, sum[k], 8 * c + 4 * e);
+          qo[k][e] = __shfl_sync(~0u, off[k], 8 * c + 4 * e);
         }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) cf[nt][u][e] = p.scale_log2 * __shfl_sync(~0u, unit[u], 8 * c + 4 * e);
-        col_pos[nt][e] = kv4_position(w.req, (int)((uint32_t)(w.rb * ROWS + nt * 8 + 2 * c + e) / (uint32_t)p.G));
+        for (int u = 0; u < NU; ++u) cf[u][e] = p.scale_log2 * __shfl_sync(~0u, unit[u], 8 * c + 4 * e);
+        col_pos[e] = kv4_position(w.req, (int)((uint32_t)(w.rb * ROWS + 2 * c + e) / (uint32_t)p.G));
       }
     }
     // Tiles in [full_lo, full_hi) are visible to every row of the block.
@@ -370,23 +369,20 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     const int full_hi = (kv4_position(w.req, (int)((uint32_t)(w.rb * ROWS) / (uint32_t)p.G)) + 1) / kTile;
     const int full_lo = p.window > 0 ? (max(0, kv4_position(w.req, last_j) - p.window + 1) + kTile - 1) / kTile : 0;
 
-    float out[NW][2][NT][4];
-    float top[NT][2], sum[NT][2], bias[NT][NG][2];
+    float out[NW][2][4];
+    float top[2], sum[2], bias[NG][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int i = 0; i < NW; ++i)
 #pragma unroll
-      for (int i = 0; i < NW; ++i)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int e = 0; e < 4; ++e) out[i][m][e] = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[i][m][nt][e] = 0.0f;
+    for (int e = 0; e < 2; ++e) {
+      top[e] = -INFINITY;
+      sum[e] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[nt][e] = -INFINITY;
-        sum[nt][e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NG; ++k) bias[nt][k][e] = 0.0f;
-      }
+      for (int k = 0; k < NG; ++k) bias[k][e] = 0.0f;
     }
 
     if (NG > 1) {
@@ -449,11 +445,11 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
               const float f = unit[grp] * reciprocal_of_power(old);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                bias[0][grp][e] *= f;
+                bias[grp][e] *= f;
 #pragma unroll
                 for (int i = grp * WPG; i < (grp + 1) * WPG; ++i)
 #pragma unroll
-                  for (int m = 0; m < 2; ++m) out[i][m][0][e] *= f, out[i][m][0][e + 2] *= f;
+                  for (int m = 0; m < 2; ++m) out[i][m][e] *= f, out[i][m][e + 2] *= f;
               }
             }
             widest = 0.0f;
@@ -493,8 +489,8 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         }
         __syncwarp();
       }
-      // ---- scores, in units of log2: s[record][nt][key g: cols, key g + 8: cols]
-      float s[2][NT][4];
+      // ---- scores, in units of log2: s[record][key g: cols, key g + 8: cols]
+      float s[2][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const uint8_t* k = rec + m * REC;
@@ -503,31 +499,24 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         lds_words<NW>(k + (g + 8) * (D / 2) + c * (D / 8), wb);
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
-          float acc[NT][4];
+          float acc[4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][e] = qo[nt][grp][e & 1];
+          for (int e = 0; e < 4; ++e) acc[e] = qo[grp][e & 1];
 #pragma unroll
           for (int i = grp * WPG; i < (grp + 1) * WPG; ++i) {
             uint32_t a0[4], a1[4];
             code_pairs(wa[i], magic_low, magic_high, a0[0], a0[2], a1[0], a1[2]);
             code_pairs(wb[i], magic_low, magic_high, a0[1], a0[3], a1[1], a1[3]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(acc[nt], a0, qf[nt][i][0], qf[nt][i][1]);
-              mma16816(acc[nt], a1, qf[nt][i][2], qf[nt][i][3]);
-            }
+            mma16816(acc, a0, qf[i][0], qf[i][1]);
+            mma16816(acc, a1, qf[i][2], qf[i][3]);
           }
           const float2 ka = pk[(m * kKv4Rec + g) * NG + grp], kb = pk[(m * kKv4Rec + g + 8) * NG + grp];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = fmaf(e < 2 ? ka.x : kb.x, acc[nt][e], (e < 2 ? ka.y : kb.y) * qs[nt][grp][e & 1]);
-              const float f = cf[nt][grp * NU / NG][e & 1];
-              s[m][nt][e] = grp ? fmaf(v, f, s[m][nt][e]) : v * f;
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float v = fmaf(e < 2 ? ka.x : kb.x, acc[e], (e < 2 ? ka.y : kb.y) * qs[grp][e & 1]);
+            const float f = cf[grp * NU / NG][e & 1];
+            s[m][e] = grp ? fmaf(v, f, s[m][e]) : v * f;
+          }
         }
       }
       const bool whole = tile >= full_lo && tile < full_hi;
@@ -535,13 +524,11 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int t = tile * kTile + m * kKv4Rec + g + (e < 2 ? 0 : 8), pos = col_pos[nt][e & 1];
-              const bool seen = t <= pos && t < len && (p.window <= 0 || t > pos - p.window);
-              if (!seen) s[m][nt][e] = -INFINITY;
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int t = tile * kTile + m * kKv4Rec + g + (e < 2 ? 0 : 8), pos = col_pos[e & 1];
+            const bool seen = t <= pos && t < len && (p.window <= 0 || t > pos - p.window);
+            if (!seen) s[m][e] = -INFINITY;
+          }
       }
       // ---- the reference exponent is that of p s, so that the weights p s are at most 2^kRoom
       float lg[2][2];  // record, key g or g + 8
@@ -551,40 +538,34 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
         for (int y = 0; y < 2; ++y) lg[m][y] = pv[(m * kKv4Rec + g + 8 * y) * NG].w;
       // ---- running reference and rescale
       bool grew = false;
-      float now[NT][2];
+      float now[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = fmaxf(fmaxf(s[0][nt][e] + lg[0][0], s[0][nt][e + 2] + lg[0][1]),
-                          fmaxf(s[1][nt][e] + lg[1][0], s[1][nt][e + 2] + lg[1][1]));
-          m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-          now[nt][e] = fmaxf(m, top[nt][e]);
-          grew |= m > top[nt][e];
-        }
+      for (int e = 0; e < 2; ++e) {
+        float m = fmaxf(fmaxf(s[0][e] + lg[0][0], s[0][e + 2] + lg[0][1]),
+                        fmaxf(s[1][e] + lg[1][0], s[1][e + 2] + lg[1][1]));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+        now[e] = fmaxf(m, top[e]);
+        grew |= m > top[e];
+      }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
+          const float f = kv4_exp2(top[e] - (now[e] == -INFINITY ? 0.0f : now[e]));
+          top[e] = now[e];
+          sum[e] *= f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float f = kv4_exp2(top[nt][e] - (now[nt][e] == -INFINITY ? 0.0f : now[nt][e]));
-            top[nt][e] = now[nt][e];
-            sum[nt][e] *= f;
+          for (int k = 0; k < NG; ++k) bias[k][e] *= f;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) bias[nt][k][e] *= f;
+          for (int i = 0; i < NW; ++i)
 #pragma unroll
-            for (int i = 0; i < NW; ++i)
-#pragma unroll
-              for (int m = 0; m < 2; ++m) out[i][m][nt][e] *= f, out[i][m][nt][e + 2] *= f;
-          }
+            for (int m = 0; m < 2; ++m) out[i][m][e] *= f, out[i][m][e + 2] *= f;
+        }
       }
-      float ref[NT][2];
+      float ref[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) ref[nt][e] = top[nt][e] == -INFINITY ? 0.0f : top[nt][e];
+      for (int e = 0; e < 2; ++e) ref[e] = top[e] == -INFINITY ? 0.0f : top[e];
       // ---- probabilities, and the products with the values
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -599,43 +580,38 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
           va[0] = v4[0], va[1] = v4[1], vb[0] = v4[2], vb[1] = v4[3];
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[m][nt][e] = kv4_exp2(s[m][nt][e] - ref[nt][e & 1]);
-            sum[nt][e & 1] += s[m][nt][e];
-          }
-        uint32_t pf[NT][NG][2];
+        for (int e = 0; e < 4; ++e) {
+          s[m][e] = kv4_exp2(s[m][e] - ref[e & 1]);
+          sum[e & 1] += s[m][e];
+        }
+        uint32_t pf[NG][2];
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
           const float4 va4 = pv[(m * kKv4Rec + g) * NG + grp], vb4 = pv[(m * kKv4Rec + g + 8) * NG + grp];
           const float r[2] = {va4.y, vb4.y}, z[2] = {va4.z, vb4.z};
+          float x[4], b[4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float x[4], b[4];
+          for (int e = 0; e < 4; ++e) x[e] = s[m][e] * (e < 2 ? va4.x : vb4.x);
+          if (!whole) {  // a key that is not seen may carry NaN parameters
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = s[m][nt][e] * (e < 2 ? va4.x : vb4.x);
-            if (!whole) {  // a key that is not seen may carry NaN parameters
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (s[m][nt][e] == 0.0f) x[e] = 0.0f;
-            }
-            const uint32_t w01 = Elem<__half>::from_f2(x[0], x[1]), w23 = Elem<__half>::from_f2(x[2], x[3]);
-            unpack2<__half>(w01, b[0], b[1]);
-            unpack2<__half>(w23, b[2], b[3]);
-            if (whole) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                bias[nt][grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][nt][e], z[e >> 1], bias[nt][grp][e & 1]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (s[m][nt][e] != 0.0f)
-                  bias[nt][grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][nt][e], z[e >> 1], bias[nt][grp][e & 1]));
-            }
-            pf[nt][grp][0] = movmatrix_trans(w01);
-            pf[nt][grp][1] = movmatrix_trans(w23);
+            for (int e = 0; e < 4; ++e)
+              if (s[m][e] == 0.0f) x[e] = 0.0f;
           }
+          const uint32_t w01 = Elem<__half>::from_f2(x[0], x[1]), w23 = Elem<__half>::from_f2(x[2], x[3]);
+          unpack2<__half>(w01, b[0], b[1]);
+          unpack2<__half>(w23, b[2], b[3]);
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              bias[grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][e], z[e >> 1], bias[grp][e & 1]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (s[m][e] != 0.0f)
+                bias[grp][e & 1] = fmaf(b[e], r[e >> 1], fmaf(s[m][e], z[e >> 1], bias[grp][e & 1]));
+          }
+          pf[grp][0] = movmatrix_trans(w01);
+          pf[grp][1] = movmatrix_trans(w23);
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
@@ -647,11 +623,8 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
             a0[e] = sub_f16x2(a0[e], e & 1 ? kCentreHigh : kCentreLow);
             a1[e] = sub_f16x2(a1[e], e & 1 ? kCentreHigh : kCentreLow);
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816(out[i][0][nt], a0, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
-            mma16816(out[i][1][nt], a1, pf[nt][i / WPG][0], pf[nt][i / WPG][1]);
-          }
+          mma16816(out[i][0], a0, pf[i / WPG][0], pf[i / WPG][1]);
+          mma16816(out[i][1], a1, pf[i / WPG][0], pf[i / WPG][1]);
         }
       }
       __syncwarp();  // every lane has read this stage
@@ -659,21 +632,16 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
-    if (!ok) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = NAN;
-    }
+    if (!ok) sum[0] = sum[1] = NAN;
     // ---- the piece's sums over the keys
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int o = 4; o < 32; o <<= 1) {
+        sum[e] += __shfl_xor_sync(~0u, sum[e], o);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          sum[nt][e] += __shfl_xor_sync(~0u, sum[nt][e], o);
-#pragma unroll
-          for (int k = 0; k < NG; ++k) bias[nt][k][e] += __shfl_xor_sync(~0u, bias[nt][k][e], o);
-        }
+        for (int k = 0; k < NG; ++k) bias[k][e] += __shfl_xor_sync(~0u, bias[k][e], o);
+      }
     float back[NG];  // from the groups' units
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) back[grp] = NG > 1 ? reciprocal_of_power(s_unit[warp][grp]) : 1.0f;
@@ -681,38 +649,36 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
     const int slot = ue == run_end;
     float* part = part_at(warp, slot);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = nt * 8 + 2 * c + e;
-        if (complete) {
-          const int row = w.rb * ROWS + col, j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
-          const float inv = sum[nt][e] > 0.0f ? 1.0f / sum[nt][e] : sum[nt][e];  // nothing seen: zeros; NaN stays
-          uint16_t* o = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + h) * D + 4 * g;
-          if (j < w.req.n) {
-#pragma unroll
-            for (int i = 0; i < NW; ++i) {
-              const float b = bias[nt][i / WPG][e], f = inv * back[i / WPG];
-              uint2 v;
-              v.x = Elem<T>::from_f2((out[i][0][nt][e] + b) * f, (out[i][0][nt][e + 2] + b) * f);
-              v.y = Elem<T>::from_f2((out[i][1][nt][e] + b) * f, (out[i][1][nt][e + 2] + b) * f);
-              *reinterpret_cast<uint2*>(o + 32 * i) = v;
-            }
-          }
-        } else {
-          if (g == 0) {
-            s_max[warp][slot][col] = top[nt][e];
-            s_sum[warp][slot][col] = sum[nt][e];
-          }
+    for (int e = 0; e < 2; ++e) {
+      const int col = 2 * c + e;
+      if (complete) {
+        const int row = w.rb * ROWS + col, j = (int)((uint32_t)row / (uint32_t)p.G), h = row - j * p.G;
+        const float inv = sum[e] > 0.0f ? 1.0f / sum[e] : sum[e];  // nothing seen: zeros; NaN stays
+        uint16_t* o = p.out + (int64_t)(w.req.start + j) * p.o_t + (int64_t)(w.kvh * p.G + h) * D + 4 * g;
+        if (j < w.req.n) {
 #pragma unroll
           for (int i = 0; i < NW; ++i) {
-            const float b = bias[nt][i / WPG][e], f = back[i / WPG];
-            *reinterpret_cast<float4*>(part + col * (D + 4) + 32 * i + 4 * g) =
-                make_float4((out[i][0][nt][e] + b) * f, (out[i][0][nt][e + 2] + b) * f, (out[i][1][nt][e] + b) * f,
-                            (out[i][1][nt][e + 2] + b) * f);
+            const float b = bias[i / WPG][e], f = inv * back[i / WPG];
+            uint2 v;
+            v.x = Elem<T>::from_f2((out[i][0][e] + b) * f, (out[i][0][e + 2] + b) * f);
+            v.y = Elem<T>::from_f2((out[i][1][e] + b) * f, (out[i][1][e + 2] + b) * f);
+            *reinterpret_cast<uint2*>(o + 32 * i) = v;
           }
         }
+      } else {
+        if (g == 0) {
+          s_max[warp][slot][col] = top[e];
+          s_sum[warp][slot][col] = sum[e];
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const float b = bias[i / WPG][e], f = back[i / WPG];
+          *reinterpret_cast<float4*>(part + col * (D + 4) + 32 * i + 4 * g) =
+              make_float4((out[i][0][e] + b) * f, (out[i][0][e + 2] + b) * f, (out[i][1][e] + b) * f,
+                          (out[i][1][e + 2] + b) * f);
+        }
       }
+    }
     if (!complete && lane == 0)
       s_info[warp][slot] = PartInfo{w.item, w.n_tiles, w.rb * ROWS, w.req.start, w.req.n, w.kvh * p.G};
     u = ue;
@@ -856,7 +822,7 @@ cudaError_t launch_t(const Kv4AttnParams& p, int sms, bool pdl, cudaStream_t str
 
 }  // namespace
 
-int64_t kv4_split_partial_bytes(int D) { return (int64_t)2 * kKv4MaxGrid * 8 * NT * (D + 2) * 4; }
+int64_t kv4_split_partial_bytes(int D) { return (int64_t)2 * kKv4MaxGrid * kRows * (D + 2) * 4; }
 
 cudaError_t launch_kv4_attn_split(const Kv4AttnParams& p, int sms, bool bf16, bool pdl, cudaStream_t stream) {
   return bf16 ? launch_t<__nv_bfloat16>(p, sms, pdl, stream) : launch_t<__half>(p, sms, pdl, stream);

@@ -319,14 +319,12 @@ __device__ __forceinline__ uint32_t kv4_opaque(uint32_t value, int not_negative)
 }
 
 // Four-bit codes as 16-bit floats: nibbles j and j + 4 of w (bits 4 j and 16 + 4 j) as the pair
-// kOffset + code, by placing the four bits in the mantissa of a constant (kOffset2, opaque).
+// offset + code, by placing the four bits in the mantissa of a constant (kOffset2, opaque).
 template <typename T>
 struct Kv4Nib;
 template <>
 struct Kv4Nib<__nv_bfloat16> {
-  static constexpr float kOffset = 128.0f;  // 0x4300: four mantissa bits of weight 1..8
-  static constexpr uint32_t kOffset2 = 0x43004300u;
-  static constexpr uint32_t kCentre2 = 0x43084308u;  // 136 = offset + 8
+  static constexpr uint32_t kOffset2 = 0x43004300u;  // 128: four mantissa bits of weight 1..8
   static constexpr bool kFullRange = true;  // of fp32
   template <int j>
   static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t magic) {
@@ -345,9 +343,7 @@ struct Kv4Nib<__nv_bfloat16> {
 };
 template <>
 struct Kv4Nib<__half> {
-  static constexpr float kOffset = 64.0f;  // 0x5400: mantissa bits 4..7 have weight 1..8
-  static constexpr uint32_t kOffset2 = 0x54005400u;
-  static constexpr uint32_t kCentre2 = 0x54805480u;  // 72 = offset + 8
+  static constexpr uint32_t kOffset2 = 0x54005400u;  // 64: mantissa bits 4..7 have weight 1..8
   static constexpr bool kFullRange = false;
   template <int j>
   static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t magic) {

@@ -27,8 +27,9 @@ from . import _lib
 from .kernel import _DTYPE_CODE, _current_device, _current_stream, _grid_workspace
 
 RECORD_TOKENS = 16
-# Query rows beyond which the library always takes its kernel for prompts (any bound is correct).
-_SPLIT_MAX_ROWS = 1024
+# Queries of a request beyond which the library always takes its kernel for prompts, and asks for
+# the same workspace.
+_ALL_PROMPTS = 1024
 
 
 class KV4Cache:
@@ -264,7 +265,7 @@ def kv4_gather(cache: KV4Cache, slots: torch.Tensor):
     return k, v
 
 
-# (n_q, n_kv, D, queries, at most 1 + the most the split kernel takes) -> bytes the library asks for.
+# (n_q, n_kv, D, queries, at most _ALL_PROMPTS + 1) -> bytes the library asks for.
 _workspace: dict = {}
 
 
@@ -352,7 +353,7 @@ def kv4_attention(
         o_t = rows.stride(0) if T > 1 else n_q * D
     if T == 0 or R == 0:
         return out.zero_()
-    key = (n_q, cache.n_kv_heads, D, min(bound, _SPLIT_MAX_ROWS + 1))
+    key = (n_q, cache.n_kv_heads, D, min(bound, _ALL_PROMPTS + 1))
     need = _workspace.get(key)
     if need is None:
         need = _workspace[key] = _lib.load().fqkv_kv4_workspace_bytes(*key)
