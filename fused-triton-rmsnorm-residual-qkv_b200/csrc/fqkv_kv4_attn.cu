@@ -25,7 +25,7 @@
 //
 // Bound: the codes' bytes over HBM, 2176 per 16 tokens and KV head at D = 128 with one group, about
 // 90 cycles of an SM's share of the bandwidth.  Measured (B200, bf16, 64 requests of 1 to 8000
-// tokens, 32 / 8 heads, 288 MB): 85 us, 3.4 TB/s; copies alone 58 us, everything but the products
+// tokens, 32 / 8 heads, 288 MB): 87 us, 3.3 TB/s; copies alone 58 us, everything but the products
 // and their unpacking 64 us.  The rest is issue: about 350 instructions a record, of which the
 // logic pipe (one per two cycles and scheduler) takes about half.
 //
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(warps<D, NG>() * 32, 2)
   __shared__ Work s_item[WARPS], s_ahead[WARPS];  // each warp's item, and the item its copies have reached
   __shared__ PartInfo s_info[WARPS][2];
   __shared__ float s_max[WARPS][2][ROWS], s_sum[WARPS][2][ROWS];
-  __shared__ float s_unit[WARPS][NG];  // each warp's powers of two that its groups' scales are multiplied by
+  __shared__ __align__(16) float s_unit[WARPS][NG];  // powers of two that a warp's groups' scales are multiplied by
   __shared__ int s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;

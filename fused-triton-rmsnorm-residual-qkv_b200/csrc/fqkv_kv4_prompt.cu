@@ -6,8 +6,9 @@
 // rescaled) when the true maximum exceeds it by 8 in the exponent; P stays below 2^8 (in bf16, whose
 // values may be as large as fp32's, below 2^-16) and the quotient O / sum does not depend on ref.
 // Keys and values are formed once per CTA as round16(scale * code + minimum), one rounding to the
-// cache's type (the operand type of the product); P is rounded to the same type, row sums, maxima
-// and accumulators are fp32.
+// cache's type (the operand type of the product), which keeps the range of the numbers and adds at
+// most an eighth to what the 4 bits lost (0.034 against 0.29 steps, root mean square, in bf16); P is
+// rounded to the same type, row sums, maxima and accumulators are fp32.
 //
 // Shape.  A CTA takes 256 query rows of one KV head (all heads that share it, so the keys are
 // unpacked once for them) as two tiles of 128 and walks the keys 128 at a time:

@@ -291,7 +291,8 @@ def kv4_attention(
             queries' own included (appended before this call).
         query_start: (R + 1,) int32, first query of each request.
         max_query_len: an upper bound of a request's queries; chooses the kernel (default: all
-            tokens with ``query_start``).
+            tokens with ``query_start``, so a batch of few queries each should pass it).  Any value is
+            correct; 1 takes the kernel for few rows, whose keys are not rounded to 16 bits.
         window: a query at position p sees p - window + 1 .. p only.
         scale: of the scores (default ``D ** -0.5``).
         out: (tokens, n_q_heads, D), rows of heads contiguous, to write into.
